@@ -277,6 +277,81 @@ SAGE3_API int sage3_selftest_bounded_wait(int32_t* device_status, void* stream);
 SAGE3_API int sage3_fp4_mma_peak(int n_cols, int bursts, int launches, int32_t* device_status, void* stream,
                                  double* tflops_out);
 
+/* ---- Serving from a 4-bit key/value cache.  No counterpart in the reference, whose operators keep nothing between calls. ----
+ *
+ * A cache is a uint8 array [num_pages, num_kv_heads, page_size / 16, 18 * D] owned by the caller, D = head_dim_stored.  A record of
+ * 18 * D bytes holds 16 tokens of one kv head: E2M1 codes of keys and values, two to a byte, with one E4M3 scale per 16 channels,
+ * in the order that csrc/kv_cache.cuh gives.  A token's slot is page * page_size + its place in the page. */
+typedef struct {
+  void* data;                /* 16-byte aligned; any contents: what is not written is never used               */
+  int64_t num_pages;
+  int32_t num_kv_heads;
+  int32_t page_size;         /* 16, 32, 64 or 128                                                              */
+  int32_t head_dim;          /* of the caller's rows: a multiple of 8, at most 128                             */
+  int32_t head_dim_stored;   /* 64 or 128, not below head_dim: channels beyond head_dim are kept as zeros      */
+  const void* k_offset;      /* optional bf16 [num_kv_heads, head_dim]: keys are stored less this vector (the channel means
+                                that K smoothing would remove; softmax does not see it, the LSE puts it back)  */
+} sage3_kv_cache;
+
+typedef struct {
+  const int32_t* lens_before;  /* device [B]: tokens of each request in the cache                              */
+  const int32_t* lens_new;     /* device [B]: tokens that this step adds                                       */
+  const int32_t* free_pages;   /* device [num_free]: page ids, handed out from the front                       */
+  int32_t* block_table;        /* device [B, columns], rows row_stride entries apart: entries of new pages are written   */
+  int64_t row_stride;
+  int32_t B, columns, num_free, page_size, num_tokens;   /* num_tokens: length of positions and slots          */
+  int32_t* kv_lens;            /* out [B]: before + new                                                        */
+  int32_t* cu_seqlens_q;       /* out [B+1]: prefix sums of new                                                */
+  int32_t* positions;          /* out [num_tokens]: place of each new token in its request; 0 behind the last  */
+  int64_t* slots;              /* out [num_tokens]: its slot; -1 where there is no page for it and behind the last       */
+  int32_t* pages_taken;        /* out [1]: pages that the step takes; more than num_free: some tokens have none          */
+} sage3_kv_tables_args;
+
+/* Per-head norm y = x * rsqrt(mean(x^2) + eps) * weight of q and k (each where its weight is given), then rotation of the first rot_dim
+ * channels by the angles of the token's position, rounded once to bf16. */
+typedef struct {
+  int32_t B, N, Hq, Hkv, D;  /* B * N tokens; D a multiple of 8, at most 128; Hq may be 0                      */
+  sage3_tensor q, k, v;      /* q.ptr or v.ptr may be NULL                                                     */
+  sage3_tensor q_out, k_out; /* k_out.ptr may be NULL where a cache is given; may be q, k themselves           */
+  const void *q_weight, *k_weight;   /* optional bf16 [D]                                                      */
+  float eps;
+  const float *cos, *sin;    /* fp32 [places, rot_dim / 2]; NULL with rot_dim 0                                */
+  int64_t places;
+  int32_t rot_dim;           /* a multiple of 8, at most D                                                     */
+  int32_t adjacent_pairs;    /* 1: channels 2i, 2i+1 form a pair; 0: i and i + rot_dim / 2                     */
+  const void* positions;     /* int32 or int64 [B, N], or NULL: token n of each batch entry is at n.  A position
+                                outside the table gives NaN                                                    */
+  int32_t positions_int64;
+  const sage3_kv_cache* cache;   /* optional: k (as rounded to bf16) and v are written to their slots          */
+  const int64_t* slots;      /* [B * N]: distinct; those outside the cache (-1) are skipped                    */
+} sage3_kv_tokens_args;
+
+typedef struct {
+  const sage3_kv_cache* cache;
+  int32_t B, Hq, max_seqlen_q, max_seqlen_k, total_q;   /* max_*: bounds on the lengths; rows of q: total_q     */
+  const void* q;             /* bf16 [total_q, Hq, head_dim], strides in elements                              */
+  int64_t q_stride_n, q_stride_h;
+  void* out;                 /* likewise; rows of no sequence stay as they are                                 */
+  int64_t out_stride_n, out_stride_h;
+  float* lse;                /* optional fp32 [total_q, Hq]                                                    */
+  const int32_t* cu_seqlens_q;   /* device [B+1], or NULL: one token per sequence                              */
+  const int32_t* kv_lens;    /* device [B]: keys of each sequence, its new tokens among them                   */
+  const int32_t* block_table;    /* device [B, columns]: page ids; keys of a page outside the cache are not seen         */
+  int64_t row_stride;
+  int32_t columns;
+  int32_t is_causal;         /* bottom-right aligned per sequence                                              */
+  float sm_scale;            /* <= 0: head_dim^-0.5                                                            */
+  void* workspace;           /* >= sage3_kv_attention_workspace bytes, 256-byte aligned; not shared by calls that can overlap  */
+  size_t workspace_bytes;
+} sage3_kv_attention_args;
+
+SAGE3_API int sage3_kv_block_tables(const sage3_kv_tables_args* args, void* stream);
+SAGE3_API int sage3_kv_tokens(const sage3_kv_tokens_args* args, void* stream);
+/* k, v: bf16 [T, num_kv_heads, head_dim], contiguous: the values that the cache stands for (with the offset); zeros for slots outside */
+SAGE3_API int sage3_kv_read(const sage3_kv_cache* cache, const int64_t* slots, int64_t T, void* k, void* v, void* stream);
+SAGE3_API int sage3_kv_attention_workspace(const sage3_kv_attention_args* args, size_t* bytes);
+SAGE3_API int sage3_kv_attention(const sage3_kv_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,10 +81,40 @@ class VarlenArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("device_status", C.c_void_p)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("num_pages", C.c_int64), ("num_kv_heads", C.c_int32), ("page_size", C.c_int32),
+                ("head_dim", C.c_int32), ("head_dim_stored", C.c_int32), ("k_offset", C.c_void_p)]
+
+
+class KvTablesArgs(C.Structure):
+    _fields_ = [("lens_before", C.c_void_p), ("lens_new", C.c_void_p), ("free_pages", C.c_void_p), ("block_table", C.c_void_p),
+                ("row_stride", C.c_int64), ("B", C.c_int32), ("columns", C.c_int32), ("num_free", C.c_int32),
+                ("page_size", C.c_int32), ("num_tokens", C.c_int32), ("kv_lens", C.c_void_p), ("cu_seqlens_q", C.c_void_p),
+                ("positions", C.c_void_p), ("slots", C.c_void_p), ("pages_taken", C.c_void_p)]
+
+
+class KvTokensArgs(C.Structure):
+    _fields_ = [("B", C.c_int32), ("N", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+                ("q", Tensor), ("k", Tensor), ("v", Tensor), ("q_out", Tensor), ("k_out", Tensor),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float), ("cos", C.c_void_p), ("sin", C.c_void_p),
+                ("places", C.c_int64), ("rot_dim", C.c_int32), ("adjacent_pairs", C.c_int32), ("positions", C.c_void_p),
+                ("positions_int64", C.c_int32), ("cache", C.POINTER(KvCache)), ("slots", C.c_void_p)]
+
+
+class KvAttentionArgs(C.Structure):
+    _fields_ = [("cache", C.POINTER(KvCache)), ("B", C.c_int32), ("Hq", C.c_int32), ("max_seqlen_q", C.c_int32),
+                ("max_seqlen_k", C.c_int32), ("total_q", C.c_int32), ("q", C.c_void_p), ("q_stride_n", C.c_int64),
+                ("q_stride_h", C.c_int64), ("out", C.c_void_p), ("out_stride_n", C.c_int64), ("out_stride_h", C.c_int64),
+                ("lse", C.c_void_p), ("cu_seqlens_q", C.c_void_p), ("kv_lens", C.c_void_p), ("block_table", C.c_void_p),
+                ("row_stride", C.c_int64), ("columns", C.c_int32), ("is_causal", C.c_int32), ("sm_scale", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 EXPORTS = ("sage3_version", "sage3_status_string", "sage3_last_cuda_error", "sage3_buffer_sizes",
            "sage3_quant_qkv", "sage3_attn_fwd", "sage3_attention", "sage3_attention_run", "sage3_attention_workspace", "sage3_attention_packed_workspace", "sage3_attention_packed_run", "sage3_read_device_status",
            "sage3_k_mean_static", "sage3_packed_rows", "sage3_packed_len", "sage3_pack_kv",
-           "sage3_attn_fwd_packed", "sage3_attention_varlen", "sage3_fp4_mma_peak", "sage3_selftest_bounded_wait")
+           "sage3_attn_fwd_packed", "sage3_attention_varlen", "sage3_fp4_mma_peak", "sage3_selftest_bounded_wait",
+           "sage3_kv_block_tables", "sage3_kv_tokens", "sage3_kv_read", "sage3_kv_attention_workspace", "sage3_kv_attention")
 
 _lib = None
 
@@ -119,6 +149,11 @@ def load() -> C.CDLL:
     lib.sage3_attention_varlen.argtypes = [C.POINTER(VarlenArgs), C.c_void_p]
     lib.sage3_fp4_mma_peak.argtypes = [C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.POINTER(C.c_double)]
     lib.sage3_selftest_bounded_wait.argtypes = [C.c_void_p, C.c_void_p]
+    lib.sage3_kv_block_tables.argtypes = [C.POINTER(KvTablesArgs), C.c_void_p]
+    lib.sage3_kv_tokens.argtypes = [C.POINTER(KvTokensArgs), C.c_void_p]
+    lib.sage3_kv_read.argtypes = [C.POINTER(KvCache), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.sage3_kv_attention_workspace.argtypes = [C.POINTER(KvAttentionArgs), C.POINTER(C.c_size_t)]
+    lib.sage3_kv_attention.argtypes = [C.POINTER(KvAttentionArgs), C.c_void_p]
     for name in EXPORTS:
         getattr(lib, name)            # raises AttributeError if an export is missing
     _lib = lib

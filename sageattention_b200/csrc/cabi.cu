@@ -10,10 +10,7 @@ namespace {
 
 thread_local int g_last_cuda_error = 0;
 
-inline int cuda_fail(cudaError_t e) {
-  g_last_cuda_error = (int)e;
-  return SAGE3_ERR_CUDA;
-}
+inline int cuda_fail(cudaError_t e) { return sage3::cuda_fail(e); }
 
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -57,6 +54,11 @@ inline size_t decode_bytes(const sage3_sizes& z, const sage3_shape& s) {
 }
 
 }  // namespace
+
+int sage3::cuda_fail(cudaError_t e) {
+  g_last_cuda_error = (int)e;
+  return SAGE3_ERR_CUDA;
+}
 
 extern "C" {
 

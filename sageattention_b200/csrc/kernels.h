@@ -8,6 +8,8 @@
 
 namespace sage3 {
 
+int cuda_fail(cudaError_t e);             // notes the error for sage3_last_cuda_error; returns SAGE3_ERR_CUDA (cabi.cu)
+
 // SMs of the current device, asked for once per device
 inline cudaError_t sm_count(int* sms) {
   static std::atomic<int> known[64];
@@ -137,5 +139,69 @@ cudaError_t launch_fp4_mma_peak(int n_cols, int bursts, int* status, cudaStream_
 
 // One CTA runs a bounded wait that must give up (selftest.cu); *status receives 77.
 cudaError_t launch_bounded_wait_selftest(int* status, cudaStream_t stream);
+
+// ---- serving from a 4-bit key/value cache (storage: kv_cache.cuh) ----
+struct KvTablesArgs {                     // block tables and slots of a step (kv_tokens.cu)
+  const int *before, *fresh;              // [B] tokens in the cache, tokens that the step adds
+  const int* free_pages;                  // [num_free] page ids, handed out in order
+  int* table;                             // [B, cols], rows table_stride apart: new entries are written
+  int64_t table_stride;
+  int B, cols, num_free, page_size, num_tokens;
+  int *kv_lens, *cu, *positions;          // [B], [B + 1], [num_tokens]
+  int64_t* slots;                         // [num_tokens]
+  int* taken;                             // [1]
+};
+cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream);
+
+struct KvRows {                           // bf16 rows, element strides
+  const void* ptr;
+  int64_t sb, sh, sn;
+};
+struct KvTokensArgs {                     // norm, rotation, cache (kv_tokens.cu)
+  KvRows q, k, vr, q_out, k_out;          // Hq == 0: no q; k_out.ptr null: k only goes to the cache
+  const void* v;                          // vr.ptr where there are values
+  int B, N, Hq, Hkv, D, DS;               // DS: 64 or 128, lanes (and stored channels) for it
+  const void* weight[2];                  // of q and k, bf16 [D], or null
+  float eps, inv_d;
+  const float *cos, *sin;                 // [places, rot / 2]
+  int64_t places;
+  int rot, adjacent;
+  const void* positions;                  // [B, N] or null: the token's number
+  int positions64;
+  uint8_t* data;                          // the cache, or null
+  const int64_t* slots;                   // [B * N]
+  const void* k_offset;
+  int page_size;
+  int64_t num_slots;
+};
+cudaError_t launch_kv_tokens(const KvTokensArgs& a, cudaStream_t stream);
+
+struct KvReadArgs {
+  const uint8_t* data;
+  const int64_t* slots;                   // [T]
+  int64_t T, num_slots;
+  int Hkv, D, DS, page_size;
+  const void* k_offset;
+  void *k, *v;                            // bf16 [T, Hkv, D]
+};
+cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream);
+
+struct KvAttnArgs {
+  const uint8_t* data;
+  int64_t num_pages;
+  int Hkv, page_size, D, DS;
+  const void *q, *k_offset;               // bf16 [tokens, Hq, D] (strides below); k_offset: for the LSE
+  void* out;
+  int64_t q_sn, q_sh, o_sn, o_sh;
+  float* lse;                             // fp32 [tokens, Hq] or null
+  const int *cu_q, *kv_lens, *table;      // cu_q null: one token per sequence
+  int64_t table_stride;
+  int B, Hq, cols, tokens, max_q, max_k, causal;
+  float sm_scale;
+  void* workspace;
+  int* status;
+};
+size_t kv_attn_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms);
+cudaError_t launch_kv_attn(const KvAttnArgs& a, cudaStream_t stream);
 
 }  // namespace sage3

@@ -1,0 +1,352 @@
+// What happens to the tokens of a step before attention over the 4-bit cache: block tables and slots, norm and rotation of queries
+// and keys, writing keys and values to the cache, and reading them back.
+#include "kernels.h"
+#include "kv_cache.cuh"
+
+namespace sage3 {
+
+// ------------------------------------------------------------------------------------------------
+// Block tables.  With have = ceil(before / ps), need = ceil((before + new) / ps) - have and their exclusive sums, new page number e of
+// the step belongs to the request that a search in the sums finds, and so does token t.  One launch: every CTA scans all requests
+// (8 bytes each, from L2) into shared memory and then takes its share of pages and tokens, so that one request with a long
+// prompt costs no more than many with short ones.  Bound by the launch: 48 requests 2.6 us, 700 requests and 1e5 tokens 4 us.
+// ------------------------------------------------------------------------------------------------
+constexpr int kTableThreads = 256;
+
+// the last i with start[i] <= x, for start[0] = 0 <= x < start[n]
+__device__ __forceinline__ int find_owner(const int* start, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const KvTablesArgs A) {
+  extern __shared__ int sm[];
+  int* const cu = sm;                     // tokens before request i
+  int* const pages = sm + A.B + 1;        // new pages before request i
+  __shared__ int2 warp_sum[kTableThreads / 32];
+  const int t = threadIdx.x, per = (A.B + kTableThreads - 1) / kTableThreads;
+  const int first = min(t * per, A.B), last = min(first + per, A.B);
+  auto lengths = [&](int i, int& before, int& fresh, int& have, int& need) {
+    before = max(__ldg(A.before + i), 0);
+    fresh = min(max(__ldg(A.fresh + i), 0), 0x7fffffff - before);
+    have = (int)(((int64_t)before + A.page_size - 1) / A.page_size);
+    need = (int)(((int64_t)before + fresh + A.page_size - 1) / A.page_size) - have;
+  };
+  int tokens = 0, wanted = 0, before, fresh, have, need;
+  for (int i = first; i < last; ++i) {
+    lengths(i, before, fresh, have, need);
+    tokens += fresh; wanted += need;
+  }
+  int2 incl = make_int2(tokens, wanted);
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int x = __shfl_up_sync(0xffffffffu, incl.x, d), y = __shfl_up_sync(0xffffffffu, incl.y, d);
+    if ((t & 31) >= d) { incl.x += x; incl.y += y; }
+  }
+  if ((t & 31) == 31) warp_sum[t >> 5] = incl;
+  __syncthreads();
+  int2 run = make_int2(incl.x - tokens, incl.y - wanted);
+  for (int w = 0; w < (t >> 5); ++w) { run.x += warp_sum[w].x; run.y += warp_sum[w].y; }
+  for (int i = first; i < last; ++i) {
+    lengths(i, before, fresh, have, need);
+    cu[i] = run.x; pages[i] = run.y;
+    run.x += fresh; run.y += need;
+    if (blockIdx.x == 0) A.kv_lens[i] = before + fresh;
+  }
+  if (t == kTableThreads - 1) {           // (the last thread's range ends at B, or is empty there)
+    cu[A.B] = run.x; pages[A.B] = run.y;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int i = t; i <= A.B; i += kTableThreads) A.cu[i] = cu[i];
+    if (t == 0) A.taken[0] = pages[A.B];
+  }
+  const int at = blockIdx.x * kTableThreads + t, step = gridDim.x * kTableThreads;
+  // new entries; the tokens below take those from the free list too, so nobody reads what is written here
+  for (int e = at; e < pages[A.B]; e += step) {
+    const int i = find_owner(pages, A.B, e);
+    lengths(i, before, fresh, have, need);
+    const int64_t col = (int64_t)have + e - pages[i];
+    if (col < A.cols) A.table[i * A.table_stride + col] = e < A.num_free ? __ldg(A.free_pages + e) : -1;
+  }
+  for (int x = at; x < A.num_tokens; x += step) {
+    int64_t slot = -1;
+    int pos = 0;
+    if (x < cu[A.B]) {
+      const int i = find_owner(cu, A.B, x);
+      lengths(i, before, fresh, have, need);
+      pos = before + x - cu[i];
+      const int col = pos / A.page_size;
+      int page = -1;
+      if (col < A.cols) {
+        if (col < have) page = A.table[i * A.table_stride + col];
+        else if (pages[i] + col - have < A.num_free) page = __ldg(A.free_pages + pages[i] + col - have);
+      }
+      if (page >= 0) slot = (int64_t)page * A.page_size + pos % A.page_size;
+    }
+    A.positions[x] = pos;
+    A.slots[x] = slot;
+  }
+}
+
+cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream) {
+  int sms;
+  if (cudaError_t e = sm_count(&sms); e != cudaSuccess) return e;
+  const int smem = 2 * (a.B + 1) * (int)sizeof(int);
+  if (smem > 48 * 1024)
+    if (cudaError_t e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return e;
+  const int64_t work = (int64_t)a.num_tokens > a.B ? a.num_tokens : a.B;
+  const int ctas = (int)((work + kTableThreads - 1) / kTableThreads);
+  block_tables_kernel<<<ctas < sms ? ctas : sms, kTableThreads, smem, stream>>>(a);
+  return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------
+// Norm, rotation, cache.  One pass: a lane has 8 channels (16 bytes) of a row, 8 or 16 lanes a row (stored head dim 64 or 128), a warp
+// kRows rows of one token's heads at a time, all loaded before the first is used.  y = x rsqrt(mean(x^2) + eps) w in fp32; channel d < R
+// is turned with its partner (d + R/2, whose lane is asked for it, or the neighbour d ^ 1) by the token's angle; one rounding to bf16.
+// To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
+// e4m3(max|x| / 6) over the two lanes of a block, code = e2m1(x / scale).  Bound by DRAM.
+// ------------------------------------------------------------------------------------------------
+constexpr int kTokenThreads = 256;
+
+// 16-channel blocks to codes and scale; a lane has half a block.  x / scale is worked out as x * (1 / scale), rounded to fp16: x has 8
+// significant bits and a border between codes times the scale 7, so a quotient that is no border is 2^-8 from it, and one that is
+// comes out as the border itself (in fp32 alone some would miss it by a last bit, 5.25 / 7 for one, and round to the other side).
+__device__ __forceinline__ void quant_half_block(const uint32_t (&x)[4], uint32_t& codes, uint32_t& scale) {
+  uint32_t m2 = abs2(habsmax2(habsmax2(x[0], x[1]), habsmax2(x[2], x[3])));
+  m2 = abs2(habsmax2(m2, __shfl_xor_sync(0xffffffffu, m2, 1)));
+  scale = f32_to_e4m3(__fdiv_rn(fmaxf(bf16_lo(m2), bf16_hi(m2)), 6.0f));
+  const float sf = e4m3_to_f32(scale), inv = sf == 0.f ? 0.f : __frcp_rn(sf);
+  float2 f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = f16x2_to_f32(pack_f16(bf16_lo(x[i]) * inv, bf16_hi(x[i]) * inv));
+  codes = f32x8_to_e2m1x8(f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y);
+}
+
+template <int DS>                         // stored head dim: 64 or 128
+__global__ void __launch_bounds__(kTokenThreads) kv_tokens_kernel(const KvTokensArgs A) {
+  using Rec = KvRecord<DS>;
+  constexpr int kLanes = DS / 8, kPerPass = 32 / kLanes, kPasses = 4, kRows = kPerPass * kPasses;
+  const int lane = threadIdx.x & 31, l = lane % kLanes, sub = lane / kLanes;
+  const int gq = (A.Hq + kRows - 1) / kRows, gk = (A.Hkv + kRows - 1) / kRows;
+  const int groups = gq + gk + (A.v != nullptr ? gk : 0);
+  const int64_t item = (int64_t)blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5);
+  const int64_t token = item / groups;
+  if (token >= (int64_t)A.B * A.N) return;
+  int g = (int)(item - token * groups);
+  const int what = g < gq ? 0 : g < gq + gk ? 1 : 2;            // q, k, v
+  g -= what == 0 ? 0 : what == 1 ? gq : gq + gk;
+  const int b = (int)(token / A.N), n = (int)(token - (int64_t)b * A.N), heads = what == 0 ? A.Hq : A.Hkv;
+  const KvRows& in = what == 0 ? A.q : what == 1 ? A.k : A.vr;
+  const __nv_bfloat16* const src = (const __nv_bfloat16*)in.ptr + b * in.sb + n * in.sn;
+  const bool have = l * 8 < A.D;                                // stored channels beyond the head dim are zero
+
+  uint4 x[kPasses];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int h = g * kRows + p * kPerPass + sub;
+    x[p] = make_uint4(0, 0, 0, 0);
+    if (have && h < heads) x[p] = __ldg(reinterpret_cast<const uint4*>(src + h * in.sh + l * 8));
+  }
+  int64_t slot = -1;
+  if (what != 0 && A.data != nullptr) {
+    slot = __ldg(A.slots + token);
+    if (slot < 0 || slot >= A.num_slots) slot = -1;
+  }
+
+  if (what != 2 && (A.weight[what] != nullptr || A.rot > 0)) {
+    const __nv_bfloat16* const weight = (const __nv_bfloat16*)A.weight[what];
+    const int quads = A.rot / 8;                                // groups of 4 channels in half of the rotated ones
+    const bool turned = l * 8 < A.rot;
+    // channels in pairs of words; the partner of group 2 l + s of 4 channels is group (2 l + s +- quads), in lane src_lane[s]
+    float w[8], cs[8], sn[8], pw[8];
+    int src_lane[2] = {lane, lane}, odd = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { w[i] = pw[i] = 1.f; cs[i] = 1.f; sn[i] = 0.f; }
+    if (weight != nullptr && have) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(weight + l * 8));
+      w[0] = bf16_lo(u.x); w[1] = bf16_hi(u.x); w[2] = bf16_lo(u.y); w[3] = bf16_hi(u.y);
+      w[4] = bf16_lo(u.z); w[5] = bf16_hi(u.z); w[6] = bf16_lo(u.w); w[7] = bf16_hi(u.w);
+    }
+    if (A.rot > 0) {
+      int64_t place = n;
+      if (A.positions != nullptr) place = A.positions64 ? __ldg((const int64_t*)A.positions + token) : (int64_t)__ldg((const int*)A.positions + token);
+      const bool known = place >= 0 && place < A.places;        // outside the table: NaN, so that it shows
+      odd = quads & 1;
+      if (turned) {
+        const int half = A.rot / 2;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int u = 2 * l + s;
+          float4 c4 = make_float4(NAN, NAN, NAN, NAN), s4 = c4;
+          if (A.adjacent) {
+            // pairs (8 l + 2 i, + 1): one angle for two channels
+            if (known && s == 0) {
+              c4 = __ldg(reinterpret_cast<const float4*>(A.cos + place * half + l * 4));
+              s4 = __ldg(reinterpret_cast<const float4*>(A.sin + place * half + l * 4));
+            }
+            if (s == 0) {
+              cs[0] = cs[1] = c4.x; cs[2] = cs[3] = c4.y; cs[4] = cs[5] = c4.z; cs[6] = cs[7] = c4.w;
+              sn[0] = -s4.x; sn[1] = s4.x; sn[2] = -s4.y; sn[3] = s4.y; sn[4] = -s4.z; sn[5] = s4.z; sn[6] = -s4.w; sn[7] = s4.w;
+            }
+          } else {
+            const bool upper = u >= quads;
+            const int pu = upper ? u - quads : u + quads;
+            if (known) {
+              c4 = __ldg(reinterpret_cast<const float4*>(A.cos + place * half + (upper ? pu : u) * 4));
+              s4 = __ldg(reinterpret_cast<const float4*>(A.sin + place * half + (upper ? pu : u) * 4));
+            }
+            const float sign = upper ? 1.f : -1.f;
+            cs[4 * s] = c4.x; cs[4 * s + 1] = c4.y; cs[4 * s + 2] = c4.z; cs[4 * s + 3] = c4.w;
+            sn[4 * s] = sign * s4.x; sn[4 * s + 1] = sign * s4.y; sn[4 * s + 2] = sign * s4.z; sn[4 * s + 3] = sign * s4.w;
+            src_lane[s] = lane - l + (pu >> 1);
+            if (weight != nullptr) {
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(weight + pu * 4));
+              pw[4 * s] = bf16_lo(v.x); pw[4 * s + 1] = bf16_hi(v.x); pw[4 * s + 2] = bf16_lo(v.y); pw[4 * s + 3] = bf16_hi(v.y);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      float f[8] = {bf16_lo(x[p].x), bf16_hi(x[p].x), bf16_lo(x[p].y), bf16_hi(x[p].y),
+                    bf16_lo(x[p].z), bf16_hi(x[p].z), bf16_lo(x[p].w), bf16_hi(x[p].w)};
+      float r = 1.f;
+      if (weight != nullptr) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf(f[i], f[i], s);
+#pragma unroll
+        for (int d = 1; d < kLanes; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+        r = 1.0f / sqrtf(s * A.inv_d + A.eps);
+      }
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = f[i] * r * w[i];
+      if (A.rot > 0) {
+        float o[8];
+        if (A.adjacent) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = y[i ^ 1];
+        } else {
+          // the partner's raw words; with an odd number of quads its other half is meant
+          uint32_t a0 = __shfl_sync(0xffffffffu, x[p].x, src_lane[0]), a1 = __shfl_sync(0xffffffffu, x[p].y, src_lane[0]);
+          uint32_t b0 = __shfl_sync(0xffffffffu, x[p].z, src_lane[1]), b1 = __shfl_sync(0xffffffffu, x[p].w, src_lane[1]);
+          if (odd) {
+            a0 = __shfl_sync(0xffffffffu, x[p].z, src_lane[0]); a1 = __shfl_sync(0xffffffffu, x[p].w, src_lane[0]);
+            b0 = __shfl_sync(0xffffffffu, x[p].x, src_lane[1]); b1 = __shfl_sync(0xffffffffu, x[p].y, src_lane[1]);
+          }
+          const float raw[8] = {bf16_lo(a0), bf16_hi(a0), bf16_lo(a1), bf16_hi(a1), bf16_lo(b0), bf16_hi(b0), bf16_lo(b1), bf16_hi(b1)};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = raw[i] * r * pw[i];
+        }
+        if (turned)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = y[i] * cs[i] + o[i] * sn[i];
+      }
+      x[p] = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+    }
+  }
+
+  const KvRows& out = what == 0 ? A.q_out : A.k_out;
+  if (what != 2 && out.ptr != nullptr && have) {
+    __nv_bfloat16* const dst = (__nv_bfloat16*)out.ptr + b * out.sb + n * out.sn;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int h = g * kRows + p * kPerPass + sub;
+      if (h < heads) *reinterpret_cast<uint4*>(dst + h * out.sh + l * 8) = x[p];
+    }
+  }
+  if (what == 0 || A.data == nullptr || slot < 0) return;       // (the whole warp: one token)
+
+  const int64_t page = slot / A.page_size;
+  const int in_page = (int)(slot - page * A.page_size), t = in_page & 15;
+  uint8_t* const base = A.data + (page * A.Hkv * (A.page_size / 16) + in_page / 16) * Rec::kBytes;
+  const int64_t head_bytes = (int64_t)(A.page_size / 16) * Rec::kBytes;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int h = g * kRows + p * kPerPass + sub;
+    uint32_t w[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
+    if (what == 1 && A.k_offset != nullptr && have && h < heads) {
+      const uint4 m = __ldg(reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.k_offset + h * A.D + l * 8));
+      const uint4 s = subtract_mean(x[p], m);
+      w[0] = s.x; w[1] = s.y; w[2] = s.z; w[3] = s.w;
+    }
+    uint32_t codes, scale;
+    quant_half_block(w, codes, scale);
+    if (h < heads) {
+      uint8_t* const rec = base + h * head_bytes;
+      *reinterpret_cast<uint32_t*>(rec + (what == 1 ? Rec::key(t, l * 8) : Rec::value(t, l * 8))) = codes;
+      if ((l & 1) == 0) rec[what == 1 ? Rec::key_scale(t, l >> 1) : Rec::value_scale(t, l >> 1)] = (uint8_t)scale;
+    }
+  }
+}
+
+cudaError_t launch_kv_tokens(const KvTokensArgs& a, cudaStream_t stream) {
+  const int rows = a.DS == 128 ? 8 : 16;
+  const int64_t groups = (a.Hq + rows - 1) / rows + (int64_t)(a.Hkv + rows - 1) / rows * (a.v != nullptr ? 2 : 1);
+  const int64_t ctas = ((int64_t)a.B * a.N * groups + kTokenThreads / 32 - 1) / (kTokenThreads / 32);
+  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  if (a.DS == 128) kv_tokens_kernel<128><<<(int)ctas, kTokenThreads, 0, stream>>>(a);
+  else kv_tokens_kernel<64><<<(int)ctas, kTokenThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------
+// Values of given slots back in bf16: code times scale (exact in bf16), keys plus their offset (rounded once).  A lane has 8 channels
+// of a row as above; slots outside the cache give zeros.
+// ------------------------------------------------------------------------------------------------
+template <int DS>
+__global__ void __launch_bounds__(kTokenThreads) kv_read_kernel(const KvReadArgs A) {
+  using Rec = KvRecord<DS>;
+  constexpr int kLanes = DS / 8;
+  const int64_t row = ((int64_t)blockIdx.x * kTokenThreads + threadIdx.x) / kLanes;
+  const int l = threadIdx.x % kLanes;
+  const int64_t token = row / A.Hkv;
+  if (token >= A.T || l * 8 >= A.D) return;
+  const int h = (int)(row - token * A.Hkv);
+  const int64_t slot = __ldg(A.slots + token);
+  uint32_t kc = 0, vc = 0, ks = 0, vs = 0;
+  if (slot >= 0 && slot < A.num_slots) {
+    const int64_t page = slot / A.page_size;
+    const int in_page = (int)(slot - page * A.page_size), t = in_page & 15;
+    const uint8_t* const rec = A.data + ((page * A.Hkv + h) * (A.page_size / 16) + in_page / 16) * Rec::kBytes;
+    kc = *reinterpret_cast<const uint32_t*>(rec + Rec::key(t, l * 8));
+    vc = *reinterpret_cast<const uint32_t*>(rec + Rec::value(t, l * 8));
+    ks = rec[Rec::key_scale(t, l >> 1)];
+    vs = rec[Rec::value_scale(t, l >> 1)];
+  }
+  uint4 off = make_uint4(0, 0, 0, 0);
+  if (A.k_offset != nullptr && slot >= 0 && slot < A.num_slots)
+    off = __ldg(reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.k_offset + h * A.D + l * 8));
+  const float kf = e4m3_to_f32(ks), vf = e4m3_to_f32(vs);
+  const uint32_t o[4] = {off.x, off.y, off.z, off.w};
+  uint32_t kh[4], vh[4];
+  e2m1x8_to_f16(kc, kh);
+  e2m1x8_to_f16(vc, vh);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 k = f16x2_to_f32(kh[i]), v = f16x2_to_f32(vh[i]);
+    kh[i] = pack_bf16(k.x * kf + bf16_lo(o[i]), k.y * kf + bf16_hi(o[i]));
+    vh[i] = pack_bf16(v.x * vf, v.y * vf);
+  }
+  const int64_t at = (token * A.Hkv + h) * A.D + l * 8;
+  *reinterpret_cast<uint4*>((__nv_bfloat16*)A.k + at) = make_uint4(kh[0], kh[1], kh[2], kh[3]);
+  *reinterpret_cast<uint4*>((__nv_bfloat16*)A.v + at) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
+}
+
+cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream) {
+  const int64_t ctas = (a.T * a.Hkv * (a.DS / 8) + kTokenThreads - 1) / kTokenThreads;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  if (a.DS == 128) kv_read_kernel<128><<<(int)ctas, kTokenThreads, 0, stream>>>(a);
+  else kv_read_kernel<64><<<(int)ctas, kTokenThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace sage3
