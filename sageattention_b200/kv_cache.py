@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .api import _as_bhnd_strides, _check_device, _on_device, _stream_ptr, _tensor_arg
+from .api import _as_bhnd_strides, _check_device, _keep_plan, _on_device, _plans, _stream_ptr
 
 _PAGE_SIZES = (16, 32, 64, 128)
 
@@ -36,10 +36,20 @@ def _check_bf16(*tensors):
 
 
 def _check_rows(*tensors):
-    """16-byte vectors: aligned start, strides of whole vectors."""
+    """16-byte vectors: strides of whole vectors (and an aligned start, which _check_aligned looks at in every call)."""
     for t in tensors:
-        _require(t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1),
-                 "every row must start on a 16-byte boundary")
+        _require(all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1), "every row must start on a 16-byte boundary")
+
+
+def _check_aligned(pointers, what):
+    if pointers & 15:
+        raise ValueError(f"{what} must start on a 16-byte boundary")
+
+
+# What a call with given shapes, strides, types and options needs is worked out once, as for the other operators (api.py): the checks and
+# the argument struct but for its pointers.  A call looks its plan up by all of these, copies the struct and fills the pointers in.
+class _Plan:
+    __slots__ = ("device", "struct", "workspace", "rows")
 
 
 def _check_ids(name, t, dtype, shape, device):
@@ -51,6 +61,28 @@ def _check_ids(name, t, dtype, shape, device):
 
 def _stored_dim(head_dim: int) -> int:
     return 64 if head_dim <= 64 else 128
+
+
+_b200 = set()
+
+
+def _check_b200(device, tensor):
+    """_check_device, asked once per device."""
+    if device not in _b200:
+        _check_device(tensor)
+        _b200.add(device)
+
+
+def _strides(x):
+    """(stride_h, stride_n) of [tokens, heads, head_dim]"""
+    return x.stride(1), x.stride(0)
+
+
+def _run(fn, struct, device, where):
+    with _on_device(device):
+        st = fn(C.byref(struct), _stream_ptr(device))
+    if st:
+        _lib.check(st, where)
 
 
 class FP4KVCache:
@@ -65,7 +97,7 @@ class FP4KVCache:
     calibrated beforehand, take the place of K smoothing (``sageattn4/api.py:184``), which would need all keys at once.  Softmax does
     not see it; :func:`sageattn_kvcache` puts it back into the log-sum-exp, :meth:`read` into the keys."""
 
-    __slots__ = ("data", "num_pages", "num_kv_heads", "page_size", "head_dim", "k_offset", "device", "_struct", "_ref")
+    __slots__ = ("data", "num_pages", "num_kv_heads", "page_size", "head_dim", "k_offset", "device", "_key", "_struct", "_ref")
 
     def __init__(self, data: torch.Tensor, head_dim: int, page_size: int = 64, k_offset: Optional[torch.Tensor] = None):
         _require(page_size in _PAGE_SIZES, f"page_size must be one of {_PAGE_SIZES}")
@@ -81,6 +113,7 @@ class FP4KVCache:
             _require(k_offset.data_ptr() % 16 == 0, "k_offset must start on a 16-byte boundary")
         self.data, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim, self.k_offset = data, pages, heads, page_size, head_dim, k_offset
         self.device = data.device
+        self._key = (pages, heads, head_dim, page_size, data.device, k_offset is None)
         self._struct = _lib.KvCache(data.data_ptr(), pages, heads, page_size, head_dim, _stored_dim(head_dim),
                                     None if k_offset is None else k_offset.data_ptr())
         self._ref = C.pointer(self._struct)
@@ -101,29 +134,39 @@ class FP4KVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Writes k, v (bf16 ``[T, num_kv_heads, head_dim]``) to the slots (int64 ``[T]``) ``page * page_size + place``.  Slots outside the cache
         (-1) are skipped; a slot named twice ends up with a mixture of its tokens."""
-        T = self._check_tokens(k, v, slots)
-        if T == 0:
-            return
-        a = _lib.KvTokensArgs()
-        a.B, a.N, a.Hq, a.Hkv, a.D = 1, T, 0, self.num_kv_heads, self.head_dim
-        a.k = _lib.Tensor(k.data_ptr(), 0, k.stride(1), k.stride(0))
-        a.v = _lib.Tensor(v.data_ptr(), 0, v.stride(1), v.stride(0))
-        a.cache, a.slots = self._ref, slots.data_ptr()
-        with _on_device(self.device):
-            _lib.check(_lib.load().sage3_kv_tokens(C.byref(a), _stream_ptr(self.device)), "sage3_kv_tokens")
+        key = ("kv_append", k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, slots.shape, slots.stride(), slots.dtype,
+               slots.device, self._key)
+        plan = _plans.get(key)
+        if plan is None:
+            T = self._check_tokens(k, v, slots)
+            plan = _Plan()
+            a = plan.struct = _lib.KvTokensArgs()
+            a.B, a.N, a.Hq, a.Hkv, a.D = 1, T, 0, self.num_kv_heads, self.head_dim
+            a.k, a.v = _lib.Tensor(None, 0, *_strides(k)), _lib.Tensor(None, 0, *_strides(v))
+            _keep_plan(key, plan)
+        kp, vp = k.data_ptr(), v.data_ptr()
+        _check_aligned(kp | vp, "k and v")
+        a = _lib.KvTokensArgs.from_buffer_copy(plan.struct)
+        a.k.ptr, a.v.ptr, a.cache, a.slots = kp, vp, self._ref, slots.data_ptr()
+        if a.N:
+            _run(_lib.load().sage3_kv_tokens, a, self.device, "sage3_kv_tokens")
 
     def read(self, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """The keys (with their offset) and values that the slots (int64 ``[T]``) stand for, bf16 ``[T, num_kv_heads, head_dim]``: for attention
         in higher precision over part of the cache, or to move tokens elsewhere.  Slots outside the cache give zeros."""
-        _require(slots.dim() == 1, "slots must be [tokens]")
-        _check_ids("slots", slots, torch.int64, slots.shape, self.device)
-        _check_device(self.data)
-        shape = (slots.shape[0], self.num_kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        with _on_device(self.device):
-            _lib.check(_lib.load().sage3_kv_read(self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(), _stream_ptr(self.device)), "sage3_kv_read")
-        return k, v
+        T = slots.shape[0] if slots.dim() == 1 else -1
+        if T < 0 or slots.dtype != torch.int64 or slots.device != self.device or not slots.is_contiguous():
+            _require(T >= 0, "slots must be [tokens]")
+            _check_ids("slots", slots, torch.int64, slots.shape, self.device)
+        dev = self.device
+        _check_b200(dev, self.data)
+        kv = torch.empty((2, T, self.num_kv_heads, self.head_dim), dtype=torch.bfloat16, device=dev)
+        p = kv.data_ptr()
+        with _on_device(dev):
+            st = _lib.load().sage3_kv_read(self._ref, slots.data_ptr(), T, p, p + kv.nbytes // 2, _stream_ptr(dev))
+        if st:
+            _lib.check(st, "sage3_kv_read")
+        return kv.unbind()
 
     def _check_tokens(self, k, v, slots):
         _check_bf16(k, v)
@@ -157,6 +200,26 @@ def build_block_tables(lens_before: torch.Tensor, lens_new: torch.Tensor, block_
     entries ``positions`` and ``slots`` get, the sum of ``lens_new`` or more (a padded batch); behind the last token slots are -1 and
     positions 0.  Nothing is read back: where the free pages or the columns do not suffice, table entries and slots are -1, and
     ``pages_taken`` says how many pages the step wanted."""
+    key = ("kv_tables", lens_before.shape, lens_before.stride(), lens_before.dtype, lens_before.device, lens_new.shape, lens_new.stride(), lens_new.dtype,
+           lens_new.device, free_pages.shape, free_pages.stride(), free_pages.dtype, free_pages.device, block_table.shape, block_table.stride(),
+           block_table.dtype, block_table.device, page_size, num_tokens)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep_plan(key, _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_tokens))
+    dev, a = plan.device, _lib.KvTablesArgs.from_buffer_copy(plan.struct)
+    B, n = a.B, a.num_tokens
+    # one allocation for all of int32
+    ints = torch.empty(2 * B + 2 + n, dtype=torch.int32, device=dev)
+    kv_lens, cu, taken, positions = ints.split((B, B + 1, 1, n))
+    slots = torch.empty(n, dtype=torch.int64, device=dev)
+    p = ints.data_ptr()
+    a.lens_before, a.lens_new, a.free_pages, a.block_table = lens_before.data_ptr(), lens_new.data_ptr(), free_pages.data_ptr(), block_table.data_ptr()
+    a.kv_lens, a.cu_seqlens_q, a.pages_taken, a.positions, a.slots = p, p + 4 * B, p + 8 * B + 4, p + 8 * B + 8, slots.data_ptr()
+    _run(_lib.load().sage3_kv_block_tables, a, dev, "sage3_kv_block_tables")
+    return BlockTables(kv_lens, cu, positions, slots, taken)
+
+
+def _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_tokens) -> _Plan:
     _require(lens_before.dim() == 1 and lens_before.shape[0] > 0, "lens_before must be [requests]")
     B, dev = lens_before.shape[0], lens_before.device
     _require(B <= 16384, "at most 16384 requests")
@@ -168,17 +231,12 @@ def build_block_tables(lens_before: torch.Tensor, lens_new: torch.Tensor, block_
     _check_ids("free_pages", free_pages, torch.int32, free_pages.shape, dev)
     _check_table(block_table, B, dev)
     _check_device(lens_before)
-    n = int(num_tokens)
-    # one allocation for all of int32
-    ints = torch.empty(2 * B + 2 + n, dtype=torch.int32, device=dev)
-    kv_lens, cu, taken, positions = ints.split((B, B + 1, 1, n))
-    slots = torch.empty(n, dtype=torch.int64, device=dev)
-    a = _lib.KvTablesArgs(lens_before.data_ptr(), lens_new.data_ptr(), free_pages.data_ptr(), block_table.data_ptr(), block_table.stride(0), B,
-                          block_table.shape[1], free_pages.shape[0], page_size, n, kv_lens.data_ptr(), cu.data_ptr(), positions.data_ptr(),
-                          slots.data_ptr(), taken.data_ptr())
-    with _on_device(dev):
-        _lib.check(_lib.load().sage3_kv_block_tables(C.byref(a), _stream_ptr(dev)), "sage3_kv_block_tables")
-    return BlockTables(kv_lens, cu, positions, slots, taken)
+    plan = _Plan()
+    plan.device = dev
+    a = plan.struct = _lib.KvTablesArgs()
+    a.row_stride, a.B, a.columns, a.num_free, a.page_size, a.num_tokens = (
+        max(block_table.stride(0), block_table.shape[1]), B, block_table.shape[1], free_pages.shape[0], page_size, int(num_tokens))
+    return plan
 
 
 def _check_table(t, B, dev):
@@ -188,13 +246,17 @@ def _check_table(t, B, dev):
     _require(B == 1 or t.stride(0) >= t.shape[1], "the rows of block_table must not overlap")
 
 
-def _norm_rope_args(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout):
-    """The argument struct of sage3_kv_tokens but for outputs and cache."""
+def _sig(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout) -> _Plan:
+    """Checks, and the argument struct of sage3_kv_tokens but for pointers, outputs and cache."""
     _check_bf16(q, k)
     _require(q.dim() == k.dim() and q.dim() in (3, 4), "q and k must be [tokens, heads, head_dim], or 4-D in tensor_layout")
     if q.dim() == 3:
         (N, Hq, D), (Nk, Hkv, Dk), B, Bk = q.shape, k.shape, 1, 1
-        qs, ks = (0, q.stride(1), q.stride(0)), (0, k.stride(1), k.stride(0))
+        qs, ks = (0, *_strides(q)), (0, *_strides(k))
         where = (N,)
     else:
         B, Hq, N, D, *qs = _as_bhnd_strides(q, tensor_layout)
@@ -205,14 +267,14 @@ def _norm_rope_args(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent
     _require(0 < D <= 128 and D % 8 == 0, f"Unsupported head_dim: {D} (a multiple of 8, at most 128)")
     _require(q.device == k.device, "q and k must be on one device")
     _check_rows(q, k)
-    a = _lib.KvTokensArgs()
+    plan = _Plan()
+    plan.device = q.device
+    a = plan.struct = _lib.KvTokensArgs()
     a.B, a.N, a.Hq, a.Hkv, a.D = B, N, Hq, Hkv, D
-    a.q, a.k = _lib.Tensor(q.data_ptr(), *qs), _lib.Tensor(k.data_ptr(), *ks)
+    a.q, a.k = _lib.Tensor(None, *qs), _lib.Tensor(None, *ks)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None:
             _check_ids(name, w, torch.bfloat16, (D,), q.device)
-            _require(w.data_ptr() % 16 == 0, f"{name} must start on a 16-byte boundary")
-            setattr(a, name, w.data_ptr())
     _require(eps >= 0, "eps must not be negative")
     a.eps = float(eps)
     _require((cos is None) == (sin is None), "cos and sin go together")
@@ -222,14 +284,38 @@ def _norm_rope_args(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent
         _require(0 < rot <= D and rot % 8 == 0, f"the rotated channels must be a multiple of 8, at most head_dim: {rot}")
         _check_ids("cos", cos, torch.float32, cos.shape, q.device)
         _check_ids("sin", sin, torch.float32, cos.shape, q.device)
-        _require(cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0, "cos and sin must start on a 16-byte boundary")
-        a.cos, a.sin, a.places, a.rot_dim, a.adjacent_pairs = cos.data_ptr(), sin.data_ptr(), cos.shape[0], rot, int(bool(adjacent_pairs))
+        a.places, a.rot_dim, a.adjacent_pairs = cos.shape[0], rot, int(bool(adjacent_pairs))
         if positions is not None:
             _require(positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64")
             _check_ids("positions", positions, positions.dtype, where, q.device)
-            a.positions, a.positions_int64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+            a.positions_int64 = int(positions.dtype == torch.int64)
     _check_device(q)
-    return a
+    return plan
+
+
+def _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight):
+    a.q.ptr, a.k.ptr = qp, kp = q.data_ptr(), k.data_ptr()
+    other = 0
+    if q_weight is not None:
+        a.q_weight = p = q_weight.data_ptr()
+        other |= p
+    if k_weight is not None:
+        a.k_weight = p = k_weight.data_ptr()
+        other |= p
+    if cos is not None:
+        a.cos, a.sin = cp, sp = cos.data_ptr(), sin.data_ptr()
+        other |= cp | sp
+        if positions is not None:
+            a.positions = positions.data_ptr()
+    _check_aligned(qp | kp, "q and k")
+    _check_aligned(other, "weights, cos and sin")
+
+
+def _check_out(o, x):
+    _check_bf16(o)
+    _require(o.shape == x.shape and o.device == x.device, "outputs must have the shapes and device of the inputs")
+    _check_rows(o)
+    _check_aligned(o.data_ptr(), "outputs")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
@@ -244,19 +330,23 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
     ``(i, i + rot_dim / 2)``, or ``(2i, 2i + 1)`` with ``adjacent_pairs``.  ``positions``: int32 or int64 ``[tokens]`` (``[batch, tokens]``), default
     0, 1, ... in each batch entry; one outside the table gives NaN.  All in fp32, rounded once.  ``out``: the two outputs, which may be q and
     k themselves."""
-    a = _norm_rope_args(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout)
-    if out is None:
-        out = torch.empty_like(q), torch.empty_like(k)
-    for o, x, name in zip(out, (q, k), ("q_out", "k_out")):
-        _check_bf16(o)
-        _require(o.shape == x.shape and o.device == x.device, "outputs must have the shapes and device of q and k")
-        _check_rows(o)
-        s = (0, o.stride(1), o.stride(0)) if o.dim() == 3 else _as_bhnd_strides(o, tensor_layout)[4:]
-        setattr(a, name, _lib.Tensor(o.data_ptr(), *s))
-    if q.shape[0] and a.N:
-        with _on_device(q.device):
-            _lib.check(_lib.load().sage3_kv_tokens(C.byref(a), _stream_ptr(q.device)), "sage3_kv_tokens")
-    return out[0], out[1]
+    if out is not None:
+        _check_out(out[0], q)
+        _check_out(out[1], k)
+    key = ("qk_norm_rope", _sig(q), _sig(k), _sig(cos), _sig(sin), _sig(positions), _sig(q_weight), _sig(k_weight), eps, adjacent_pairs, tensor_layout)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep_plan(key, _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout))
+    a = _lib.KvTokensArgs.from_buffer_copy(plan.struct)
+    _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight)
+    yq, yk = (torch.empty_like(q), torch.empty_like(k)) if out is None else out
+    if q.dim() == 3:
+        a.q_out, a.k_out = _lib.Tensor(yq.data_ptr(), 0, *_strides(yq)), _lib.Tensor(yk.data_ptr(), 0, *_strides(yk))
+    else:
+        a.q_out, a.k_out = (_lib.Tensor(y.data_ptr(), *_as_bhnd_strides(y, tensor_layout)[4:]) for y in (yq, yk))
+    if a.B and a.N:
+        _run(_lib.load().sage3_kv_tokens, a, plan.device, "sage3_kv_tokens")
+    return yq, yk
 
 
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: FP4KVCache, slots: torch.Tensor,
@@ -266,21 +356,27 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`qk_norm_rope` of ``[tokens, heads, head_dim]`` tensors with the keys, and the values as they are, written straight to the cache
     (the same bits as :meth:`FP4KVCache.append` of its result).  Returns the queries."""
-    _require(q.dim() == 3, "q must be [tokens, heads, head_dim]")
-    a = _norm_rope_args(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, "NHD")
-    cache._check_tokens(k, v, slots)
-    _require(q.device == cache.device, "q and the cache must be on one device")
+    if out is not None:
+        _check_out(out, q)
+    key = ("qk_norm_rope_append", _sig(q), _sig(k), _sig(v), _sig(slots), _sig(cos), _sig(sin), _sig(positions), _sig(q_weight), _sig(k_weight), eps,
+           adjacent_pairs, cache._key)
+    plan = _plans.get(key)
+    if plan is None:
+        _require(q.dim() == 3, "q must be [tokens, heads, head_dim]")
+        plan = _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, "NHD")
+        cache._check_tokens(k, v, slots)
+        _require(q.device == cache.device, "q and the cache must be on one device")
+        plan.struct.v = _lib.Tensor(None, 0, *_strides(v))
+        _keep_plan(key, plan)
+    a = _lib.KvTokensArgs.from_buffer_copy(plan.struct)
+    _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight)
     if out is None:
         out = torch.empty_like(q)
-    _check_bf16(out)
-    _require(out.shape == q.shape and out.device == q.device, "out must have the shape and device of q")
-    _check_rows(out)
-    a.q_out = _lib.Tensor(out.data_ptr(), 0, out.stride(1), out.stride(0))
-    a.v = _lib.Tensor(v.data_ptr(), 0, v.stride(1), v.stride(0))
-    a.cache, a.slots = cache._ref, slots.data_ptr()
+    vp = v.data_ptr()
+    _check_aligned(vp, "v")
+    a.q_out, a.v.ptr, a.cache, a.slots = _lib.Tensor(out.data_ptr(), 0, *_strides(out)), vp, cache._ref, slots.data_ptr()
     if a.N:
-        with _on_device(q.device):
-            _lib.check(_lib.load().sage3_kv_tokens(C.byref(a), _stream_ptr(q.device)), "sage3_kv_tokens")
+        _run(_lib.load().sage3_kv_tokens, a, plan.device, "sage3_kv_tokens")
     return out
 
 
@@ -300,6 +396,32 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     LSE of ``-inf``; keys of pages outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not
     touched in ``out`` (or are undefined in a new tensor).  Returns the output like q, and with ``return_lse`` the natural-log LSE fp32
     ``[tokens, Hq]`` of ``sm_scale * q.k``."""
+    if out is not None:
+        _check_out(out, q)
+    key = ("kvcache", _sig(q), cache._key, _sig(block_table), _sig(kv_lens), _sig(cu_seqlens_q), max_seqlen_q, max_seqlen_k, bool(is_causal), sm_scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep_plan(key, _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, is_causal, sm_scale))
+    dev, a = plan.device, _lib.KvAttentionArgs.from_buffer_copy(plan.struct)
+    if out is None:
+        out = torch.empty_like(q)
+    lse = torch.empty(plan.rows, dtype=torch.float32, device=dev) if return_lse else None
+    if a.total_q:
+        ws = torch.empty(plan.workspace, dtype=torch.uint8, device=dev)
+        qp = q.data_ptr()
+        _check_aligned(qp, "q")
+        a.cache, a.q, a.out, a.kv_lens, a.block_table = cache._ref, qp, out.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr()
+        a.out_stride_h, a.out_stride_n = _strides(out)
+        if lse is not None:
+            a.lse = lse.data_ptr()
+        if cu_seqlens_q is not None:
+            a.cu_seqlens_q = cu_seqlens_q.data_ptr()
+        a.workspace = ws.data_ptr()
+        _run(_lib.load().sage3_kv_attention, a, dev, "sage3_kv_attention")
+    return (out, lse) if return_lse else out
+
+
+def _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, is_causal, sm_scale) -> _Plan:
     _check_bf16(q)
     _require(q.dim() == 3 and q.shape[2] == cache.head_dim, f"q must be [tokens, heads, {cache.head_dim}]")
     T, Hq, _ = q.shape
@@ -321,23 +443,19 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     _require(max_seqlen_k > 0, "max_seqlen_k must be positive")
     _require(sm_scale is None or sm_scale > 0, "sm_scale must be positive")
     _check_rows(q)
-    if out is None:
-        out = torch.empty_like(q)
-    _check_bf16(out)
-    _require(out.shape == q.shape and out.device == dev, "out must have the shape and device of q")
-    _check_rows(out)
     _check_device(q)
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
-    if T:
-        lib = _lib.load()
-        a = _lib.KvAttentionArgs(cache._ref, B, Hq, int(max_seqlen_q), int(max_seqlen_k), T, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
-                                 out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
-                                 None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(),
-                                 block_table.stride(0), block_table.shape[1], int(bool(is_causal)), 0.0 if sm_scale is None else float(sm_scale))
-        with _on_device(dev):
-            n = C.c_size_t()
-            _lib.check(lib.sage3_kv_attention_workspace(C.byref(a), C.byref(n)), "sage3_kv_attention_workspace")
-            ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
-            _lib.check(lib.sage3_kv_attention(C.byref(a), _stream_ptr(dev)), "sage3_kv_attention")
-    return (out, lse) if return_lse else out
+    plan = _Plan()
+    plan.device, plan.rows = dev, (T, Hq)
+    a = plan.struct = _lib.KvAttentionArgs()
+    a.B, a.Hq, a.max_seqlen_q, a.max_seqlen_k, a.total_q = B, Hq, int(max_seqlen_q), max_seqlen_k, T
+    a.q_stride_h, a.q_stride_n = _strides(q)
+    a.row_stride, a.columns, a.is_causal = block_table.stride(0), block_table.shape[1], int(bool(is_causal))
+    a.sm_scale = 0.0 if sm_scale is None else float(sm_scale)
+    # the size of the workspace goes by the sizes alone; a pointer says whether there are offsets
+    a.cache, a.cu_seqlens_q = cache._ref, None if cu_seqlens_q is None else cu_seqlens_q.data_ptr()
+    n = C.c_size_t()
+    with _on_device(dev):
+        _lib.check(_lib.load().sage3_kv_attention_workspace(C.byref(a), C.byref(n)), "sage3_kv_attention_workspace")
+    a.cache, a.cu_seqlens_q = None, None
+    plan.workspace = a.workspace_bytes = n.value
+    return plan

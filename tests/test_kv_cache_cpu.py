@@ -172,7 +172,7 @@ def attention_args(**kw):
     (dict(max_seqlen_k=0), ValueError, "max_seqlen_k"),
     (dict(block_table=torch.zeros(1, 1, dtype=torch.int32)), ValueError, "block_table"),
     (dict(sm_scale=-0.1), ValueError, "sm_scale"),
-    (dict(out=tokens(T=2, H=2)), ValueError, "out must have"),
+    (dict(out=tokens(T=2, H=2)), ValueError, "outputs must have"),
     (dict(), ValueError, "CUDA tensors only"),
 ])
 def test_attention_refusals(kw, exc, match):
