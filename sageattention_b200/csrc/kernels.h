@@ -202,6 +202,7 @@ struct KvAttnArgs {
   int* status;
 };
 size_t kv_attn_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms);
+bool kv_attn_fits(int B, int Hq, int Hkv, int max_q, int max_k);    // its counts stay within 32 bits
 cudaError_t launch_kv_attn(const KvAttnArgs& a, cudaStream_t stream);
 
 }  // namespace sage3

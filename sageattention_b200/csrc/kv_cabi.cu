@@ -34,9 +34,9 @@ int check_attention(const sage3_kv_attention_args* a) {
   if (int st = check_cache(a->cache)) return st;
   if (a->B <= 0 || a->Hq <= 0 || a->max_seqlen_q <= 0 || a->max_seqlen_k <= 0 || a->total_q < 0 || a->columns <= 0) return SAGE3_ERR_ARGUMENT;
   if (a->Hq % a->cache->num_kv_heads != 0) return SAGE3_ERR_UNSUPPORTED;
-  // rows of a kv head and (sequence, kv head) pairs are counted in 32 bits, tiles of rows in a grid dimension of 16
-  const int64_t rows = (int64_t)a->max_seqlen_q * (a->Hq / a->cache->num_kv_heads);
-  if (rows > 8 * 65535 || (int64_t)a->B * a->cache->num_kv_heads >= (1ll << 31) || a->max_seqlen_k > (1 << 30)) return SAGE3_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)longest_q(a) * (a->Hq / a->cache->num_kv_heads);
+  if (rows >= (1ll << 30) || a->max_seqlen_k > (1 << 30) || !sage3::kv_attn_fits(a->B, a->Hq, a->cache->num_kv_heads, longest_q(a), a->max_seqlen_k))
+    return SAGE3_ERR_UNSUPPORTED;
   return SAGE3_OK;
 }
 

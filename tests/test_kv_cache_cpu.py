@@ -241,7 +241,7 @@ def test_c_entry_points_check_arguments():
         return lib.sage3_kv_attention(C.byref(a), None)
 
     for bad, want in ((dict(Hq=3), U), (dict(B=0), A), (dict(max_seqlen_k=0), A), (dict(columns=0), A), (dict(q=None), A), (dict(q=one + 2), A), (dict(kv_lens=None), A),
-                      (dict(q_stride_n=250), A), (dict(workspace=one + 16), A), (dict(total_q=0), _lib.OK), (dict(B=2), A), (dict(cu_seqlens_q=one, max_seqlen_q=1 << 20), U)):
+                      (dict(q_stride_n=250), A), (dict(workspace=one + 16), A), (dict(total_q=0), _lib.OK), (dict(B=2), A), (dict(cu_seqlens_q=one, max_seqlen_q=1 << 30), U)):
         assert att(**bad) == want, bad
     t = _lib.KvTablesArgs(one, one, one, one, 4, 2, 4, 1, 16, 2, one, one, one, one, one)
     for n, x, want in (("B", 0, A), ("B", 20000, U), ("columns", 5, A), ("page_size", 17, U), ("num_free", -1, A), ("free_pages", None, A), ("slots", None, A)):
