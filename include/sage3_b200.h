@@ -343,6 +343,7 @@ typedef struct {
   float sm_scale;            /* <= 0: head_dim^-0.5                                                            */
   void* workspace;           /* >= sage3_kv_attention_workspace bytes, 256-byte aligned; not shared by calls that can overlap  */
   size_t workspace_bytes;
+  int32_t* device_status;    /* optional device int32, zeroed by the call: the code of a bounded wait that gave up       */
 } sage3_kv_attention_args;
 
 SAGE3_API int sage3_kv_block_tables(const sage3_kv_tables_args* args, void* stream);

@@ -107,7 +107,7 @@ class KvAttentionArgs(C.Structure):
                 ("q_stride_h", C.c_int64), ("out", C.c_void_p), ("out_stride_n", C.c_int64), ("out_stride_h", C.c_int64),
                 ("lse", C.c_void_p), ("cu_seqlens_q", C.c_void_p), ("kv_lens", C.c_void_p), ("block_table", C.c_void_p),
                 ("row_stride", C.c_int64), ("columns", C.c_int32), ("is_causal", C.c_int32), ("sm_scale", C.c_float),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("device_status", C.c_void_p)]
 
 
 EXPORTS = ("sage3_version", "sage3_status_string", "sage3_last_cuda_error", "sage3_buffer_sizes",

@@ -29,13 +29,19 @@ sage3::KvRows rows_of(const sage3_tensor& t) { return sage3::KvRows{t.ptr, t.str
 // without offsets every sequence has one token
 inline int longest_q(const sage3_kv_attention_args* a) { return a->cu_seqlens_q != nullptr ? a->max_seqlen_q : 1; }
 
+inline bool takes_prefill(const sage3_kv_attention_args* a) {
+  return sage3::kv_prefill_takes(a->Hq, a->cache->num_kv_heads, a->cache->head_dim_stored, longest_q(a), a->max_seqlen_k);
+}
+
 int check_attention(const sage3_kv_attention_args* a) {
   if (a == nullptr) return SAGE3_ERR_ARGUMENT;
   if (int st = check_cache(a->cache)) return st;
   if (a->B <= 0 || a->Hq <= 0 || a->max_seqlen_q <= 0 || a->max_seqlen_k <= 0 || a->total_q < 0 || a->columns <= 0) return SAGE3_ERR_ARGUMENT;
   if (a->Hq % a->cache->num_kv_heads != 0) return SAGE3_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)longest_q(a) * (a->Hq / a->cache->num_kv_heads);
-  if (rows >= (1ll << 30) || a->max_seqlen_k > (1 << 30) || !sage3::kv_attn_fits(a->B, a->Hq, a->cache->num_kv_heads, longest_q(a), a->max_seqlen_k))
+  if (rows >= (1ll << 30) || a->max_seqlen_k > (1 << 30)) return SAGE3_ERR_UNSUPPORTED;
+  if (takes_prefill(a) ? !sage3::kv_prefill_fits(a->B, a->Hq, a->cache->num_kv_heads, longest_q(a))
+                       : !sage3::kv_decode_fits(a->B, a->Hq, a->cache->num_kv_heads, longest_q(a), a->max_seqlen_k))
     return SAGE3_ERR_UNSUPPORTED;
   return SAGE3_OK;
 }
@@ -112,7 +118,8 @@ int sage3_kv_attention_workspace(const sage3_kv_attention_args* a, size_t* bytes
   if (bytes == nullptr) return SAGE3_ERR_ARGUMENT;
   int sms;
   if (cudaError_t e = sage3::sm_count(&sms); e != cudaSuccess) return sage3::cuda_fail(e);
-  *bytes = sage3::kv_attn_workspace(a->B, a->Hq, a->cache->num_kv_heads, a->cache->head_dim_stored, longest_q(a), a->max_seqlen_k, sms);
+  const auto size = takes_prefill(a) ? sage3::kv_prefill_workspace : sage3::kv_decode_workspace;
+  *bytes = size(a->B, a->Hq, a->cache->num_kv_heads, a->cache->head_dim_stored, longest_q(a), a->max_seqlen_k, sms);
   return SAGE3_OK;
 }
 
@@ -136,8 +143,10 @@ int sage3_kv_attention(const sage3_kv_attention_args* a, void* stream) {
   k.B = a->B; k.Hq = a->Hq; k.cols = a->columns; k.tokens = a->total_q;
   k.max_q = longest_q(a); k.max_k = a->max_seqlen_k; k.causal = a->is_causal != 0;
   k.sm_scale = a->sm_scale > 0.f ? a->sm_scale : 1.0f / sqrtf((float)c.head_dim);
-  k.workspace = a->workspace;
-  cudaError_t e = sage3::launch_kv_attn(k, (cudaStream_t)stream);
+  k.workspace = a->workspace; k.status = a->device_status;
+  cudaError_t e = cudaSuccess;
+  if (a->device_status != nullptr) e = cudaMemsetAsync(a->device_status, 0, sizeof(int32_t), (cudaStream_t)stream);
+  if (e == cudaSuccess) e = takes_prefill(a) ? sage3::launch_kv_prefill(k, (cudaStream_t)stream) : sage3::launch_kv_decode(k, (cudaStream_t)stream);
   return e == cudaSuccess ? SAGE3_OK : sage3::cuda_fail(e);
 }
 

@@ -12,16 +12,13 @@
 // The four, and then parts of a row that several CTAs have (a second small kernel, launched as a programmatic dependent), are joined
 // by their maxima and sums in a fixed order.
 #include "kernels.h"
-#include "kv_cache.cuh"
+#include "kv_attn.cuh"
 
 namespace sage3 {
 
 namespace {
 
 constexpr int kWarps = 4, kChunk = 32, kStages = 3, kBlock = kWarps * kChunk;
-constexpr float kTop = 8.f;               // log2 of P where a score is the row's maximum
-constexpr float kSlack = 7.f;             // by which later scores may pass it before anything is rescaled: P stays below 2^15
-constexpr float kLowest = -1e38f;         // the maximum of a row that has seen no key
 
 struct Header {                           // at the front of the workspace, for the joining kernel
   int per;                                // units of work per CTA
@@ -77,23 +74,10 @@ __device__ __forceinline__ uint32_t lds16(uint32_t at) {
   return v;
 }
 
-// Where a sequence's rows and keys lie; every bound that memory accesses rely on is taken here.
-struct Seq {
-  int q0, q_len, kv_len;
-  __device__ __forceinline__ Seq(const KvAttnArgs& A, int b) {
-    q0 = b; q_len = 1;
-    if (A.cu_q != nullptr) { q0 = __ldg(A.cu_q + b); q_len = __ldg(A.cu_q + b + 1) - q0; }
-    if (q0 < 0 || q_len < 0 || q0 > A.tokens) { q0 = 0; q_len = 0; }
-    q_len = min(min(q_len, A.max_q), A.tokens - q0);
-    kv_len = (int)min((int64_t)max(__ldg(A.kv_lens + b), 0), (int64_t)A.cols * A.page_size);
-    kv_len = min(kv_len, A.max_k);
-  }
-  // 128-key blocks of an item (one at least, so that rows without keys are written too) and items per kv head
-  __device__ __forceinline__ int blocks() const { return max(1, (kv_len + kBlock - 1) / kBlock); }
-  __device__ __forceinline__ int tiles(int group, int rows) const { return (q_len * group + rows - 1) / rows; }
-  // keys that token t of the sequence sees
-  __device__ __forceinline__ int seen(const KvAttnArgs& A, int t) const { return A.causal ? max(0, min(kv_len, kv_len - q_len + t + 1)) : kv_len; }
-};
+// 128-key blocks of an item (one at least, so that rows without keys are written too) and items per kv head
+__device__ __forceinline__ int blocks_of(const KvSeq& s) { return max(1, (s.kv_len + kBlock - 1) / kBlock); }
+template <int kRows>
+__device__ __forceinline__ int tiles_of(const KvSeq& s, int group) { return (s.q_len * group + kRows - 1) / kRows; }
 
 template <int D, int NB>
 constexpr int smem_bytes() {
@@ -122,8 +106,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(co
 
   // ---- this CTA's units
   auto units = [&](int b) {
-    const Seq s(A, b);
-    return A.Hkv * s.tiles(P.group, kRows) * s.blocks();
+    const KvSeq s(A, b);
+    return A.Hkv * tiles_of<kRows>(s, P.group) * blocks_of(s);
   };
   int total = 0;
   for (int b = threadIdx.x; b < A.B; b += kWarps * 32) total += units(b);
@@ -164,8 +148,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(co
 
 #pragma unroll 1
   while (unit < unit_end) {
-    const Seq seq(A, b);
-    const int blocks = seq.blocks(), tiles = seq.tiles(P.group, kRows);
+    const KvSeq seq(A, b);
+    const int blocks = blocks_of(seq), tiles = tiles_of<kRows>(seq, P.group);
     if (rest >= A.Hkv * tiles * blocks) {             // on to the next sequence
       rest -= A.Hkv * tiles * blocks;
       if (++b >= A.B) break;
@@ -247,9 +231,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(co
       float m = fmaxf(bf16_lo(m2), bf16_hi(m2));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      // 2^(14 - exponent), within the normal numbers
-      const int field = min(268 - (int)(__float_as_uint(m) >> 23), 253);
-      const float up = __uint_as_float((uint32_t)field << 23), undo = __uint_as_float((uint32_t)(254 - field) << 23);
+      const RowScale scale(m);
+      const float up = scale.up, undo = scale.undo;
 #pragma unroll
       for (int i = 0; i < kKS; ++i) {
         qf[r][i][0] = pack_f16(bf16_lo(w[2 * i]) * up, bf16_hi(w[2 * i]) * up);
@@ -504,7 +487,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(co
             *reinterpret_cast<uint2*>(out + ch + k) =
                 make_uint2(pack_bf16(acc[k] * inv, acc[k + 1] * inv), pack_bf16(acc[k + 2] * inv, acc[k + 3] * inv));
         if (ch == 0 && A.lse != nullptr)
-          A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = l == 0.f ? -INFINITY : (m - kTop + log2f(l)) * 0.6931471805599453f + add_s[row];
+          A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, add_s[row]);
       } else {
         const int64_t at = ((int64_t)blockIdx.x * 2 + (head_of_item ? 1 : 0)) * kRows + row;
 #pragma unroll
@@ -531,12 +514,12 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const Params P) {
   const int row_id = id % kRows, bh = item / P.tiles, tile = item - bh * P.tiles;
   if (bh >= A.B * A.Hkv) return;                                // (a whole warp; others of the CTA wait below)
   const int b = bh / A.Hkv, h = bh - b * A.Hkv;
-  const Seq seq(A, b);
+  const KvSeq seq(A, b);
   const int row = tile * kRows + row_id;
   pdl_wait();                              // also where there is no row: what follows on the stream may write the first kernel's inputs
   if (row >= seq.q_len * P.group) return;
   const int start = P.item_start[item], per = P.header->per;
-  const int first = start / per, last = (start + seq.blocks() - 1) / per;
+  const int first = start / per, last = (start + blocks_of(seq) - 1) / per;
   if (first == last) return;
   // the first CTA had the item last, the others had it first
   auto place = [&](int cta) { return ((int64_t)cta * 2 + (cta == first ? 1 : 0)) * kRows + row_id; };
@@ -569,7 +552,7 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const Params P) {
     for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16(acc[i] * inv, acc[i + 1] * inv);
   }
   if (lane == 0 && A.lse != nullptr)
-    A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = l == 0.f ? -INFINITY : (m - kTop + log2f(l)) * 0.6931471805599453f + P.lse_add[(int64_t)item * kRows + row_id];
+    A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, P.lse_add[(int64_t)item * kRows + row_id]);
 }
 
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -612,18 +595,18 @@ cudaError_t launch(const Params& P, const Plan& p, bool split, cudaStream_t stre
 
 }  // namespace
 
-size_t kv_attn_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) { return plan(B, Hq, Hkv, DS, max_q, max_k, sms).bytes; }
+size_t kv_decode_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) { return plan(B, Hq, Hkv, DS, max_q, max_k, sms).bytes; }
 
-bool kv_attn_fits(int B, int Hq, int Hkv, int max_q, int max_k) {
+bool kv_decode_fits(int B, int Hq, int Hkv, int max_q, int max_k) {
   const Plan p = plan(B, Hq, Hkv, 128, max_q, max_k, 1);
   return p.units < (1ll << 30) && p.rows < (1ll << 30);
 }
 
-cudaError_t launch_kv_attn(const KvAttnArgs& a, cudaStream_t stream) {
+cudaError_t launch_kv_decode(const KvAttnArgs& a, cudaStream_t stream) {
   int sms;
   if (cudaError_t e = sm_count(&sms); e != cudaSuccess) return e;
   const Plan p = plan(a.B, a.Hq, a.Hkv, a.DS, a.max_q, a.max_k, sms);
-  if (p.units >= (1ll << 30) || p.rows >= (1ll << 30)) return cudaErrorInvalidValue;      // (kv_attn_fits has said so)
+  if (p.units >= (1ll << 30) || p.rows >= (1ll << 30)) return cudaErrorInvalidValue;      // (kv_decode_fits has said so)
   Params P;
   P.a = a;
   P.group = a.Hq / a.Hkv; P.tiles = p.tiles;

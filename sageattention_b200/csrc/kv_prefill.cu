@@ -1,0 +1,647 @@
+// Attention of many query rows per kv head over the 4-bit cache: chunks of prompts behind cached prefixes.
+//
+// A CTA takes 256 rows (tokens times the heads of a kv head, two tiles of 128) of a (sequence, kv head) and walks tiles of 128 keys:
+//   warps 8-11   read records of the cache as they are, turn codes and scales into fp16 (exact, see kv_decode.cu) and write K and V tiles
+//                to shared memory, once for all 256 rows.  Both lie alike, rows of keys with 128-byte swizzle: K is then the K-major B
+//                operand of S = Q K^T and V the MN-major one of O += P V, so nothing is transposed
+//   warp  12     issues the tcgen05.mma kind::f16: S_t = Q_t K^T (queries from shared memory), O_t += P_t V (P from tensor memory)
+//   warps 0-3    softmax of row tile 0, a thread per row: scores from tensor memory to registers, weights back over them in fp16
+//   warps 4-7    the same for row tile 1; one tile's softmax runs beside the other's MMAs
+// A row's maximum is brought up to date only where a score passes it by 2^7 (kv_attn.cuh); then its thread rescales the row of O.
+// With few items the keys are split over CTAs as well and joined by a second kernel.
+//
+// Tensor memory (512 columns): S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t takes the first 64 columns of S_t:
+// the MMAs are executed in the order of their issue, so Q_t K^T of the next key tile comes behind the P_t V that reads them.
+//
+// Every wait on an mbarrier is bounded; where one gives up the CTA records its code in *status, waits (bounded) for its MMAs in
+// flight, frees its tensor memory and returns: 60 K stage free, 61 V stage free, 62 Q there, 63 K there, 64 V there, 65 P there, 66 scores
+// there, 67 last P V done.
+#include "kv_attn.cuh"
+
+namespace sage3 {
+
+namespace {
+
+constexpr int kThreads2 = 512, kM = 128, kN = 128, kItemRows = 2 * kM;
+// Register hand-over (setmaxnreg) moves registers inside the pool the CTA was launched with, 128 a thread; launch() checks that.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kFillRegs = 80, kRoleRegs = 48;
+static_assert(256 * kSoftmaxRegs + 128 * (kFillRegs + kRoleRegs) <= kThreads2 * kLaunchRegs, "setmaxnreg split exceeds the CTA's register pool");
+
+template <int D>
+struct Lay {                              // shared memory
+  static constexpr int kOperand = kM * D * 2, kHalf = kM * 128;      // a tile; its part of 64 channels
+  static constexpr int q = 0, k = 2 * kOperand, v = 4 * kOperand, bars = 6 * kOperand, total = bars + 256;
+  // 16 bytes: channels 8 chunk ... of a row
+  static __device__ __forceinline__ int at(int row, int chunk) { return (chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
+};
+struct Bar {                              // byte offsets in the barrier block, two of each
+  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96, pv_done = 112, drain = 128, tmem = 144, abort = 152;
+};
+
+struct Params2 {
+  KvAttnArgs a;
+  int group, tiles, splits, page_shift;
+  float scale_log2;
+  int* status;
+  float* o_part;                          // [split, B * Hkv, tiles, 256, DS]
+  float2* ml_part;                        // [split, B * Hkv, tiles, 256]: maximum (log2) and sum
+  float* lse_add;                         // [B * Hkv, tiles, 256]
+};
+
+// Key tiles that the two row tiles of an item see, and a split's share of them
+struct Range {
+  int n[2], first, count[2];
+  __device__ __forceinline__ Range(const KvSeq& seq, const Params2& P, int row0, int rows, int split) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r0 = row0 + t * kM;
+      n[t] = r0 < rows ? (seq.seen(P.a, (min(rows, r0 + kM) - 1) / P.group) + kN - 1) / kN : 0;
+    }
+    const int all = max(n[0], n[1]), per = (all + P.splits - 1) / P.splits;
+    first = min(split * per, all);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) count[t] = max(0, min(min(first + per, all), n[t]) - first);
+  }
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %5, 0;\nmov.b64 da, {%1, %3};\nmov.b64 db, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 db;\nsetp.ne.b32 p, %5, 0;\nmov.b64 db, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}" ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&x)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+}
+__device__ __forceinline__ uint32_t splat(uint32_t pair, bool hi) { return __byte_perm(pair, 0, hi ? 0x3232 : 0x1010); }
+
+// fp16 x fp16 -> fp32, A K-major, B K-major or (transposed) MN-major
+__host__ __device__ constexpr uint32_t idesc_f16(int N, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kM >> 4) << 24); }
+
+template <int D>
+__global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 P) {
+  using Rec = KvRecord<D>;
+  using L = Lay<D>;
+  extern __shared__ uint8_t raw[];
+  const KvAttnArgs& A = P.a;
+  uint8_t* const smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  const uint32_t base = smem_u32(smem), bars = base + L::bars;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  volatile int* const abort_s = reinterpret_cast<volatile int*>(smem + L::bars + Bar::abort);
+  pdl_launch_dependents();
+
+  // ---- the item: the last rows, which see the most keys, first
+  const int heads = A.B * A.Hkv, bh = blockIdx.x % heads, tile = P.tiles - 1 - (int)(blockIdx.x / heads), split = blockIdx.y;
+  const int b = bh / A.Hkv, h = bh - b * A.Hkv;
+  const KvSeq seq(A, b);
+  const int rows = seq.q_len * P.group, row0 = tile * kItemRows;
+  if (row0 >= rows) return;
+  const Range R(seq, P, row0, rows, split);
+  const int steps = max(R.count[0], R.count[1]);
+  if (steps == 0 && P.splits > 1) return;                      // (the joining kernel knows)
+  const int see_any = seq.seen(A, (min(rows, row0 + kItemRows) - 1) / P.group);
+  const int* const table = A.table + b * A.table_stride;
+  const int key_begin = R.first * kN, key_end = min((R.first + steps) * kN, see_any);
+  auto has_page = [&](int key) { return (uint32_t)__ldg(table + (key >> P.page_shift)) < (uint64_t)A.num_pages; };
+  int absent = 0;
+  for (int key = key_begin + (int)threadIdx.x * A.page_size; key < key_end; key += kThreads2 * A.page_size) absent |= !has_page(key);
+
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + Bar::k_full + 8 * i, 4);
+      mbar_init(bars + Bar::k_empty + 8 * i, 1);
+      mbar_init(bars + Bar::v_full + 8 * i, 4);
+      mbar_init(bars + Bar::v_empty + 8 * i, 1);
+      mbar_init(bars + Bar::q_full + 8 * i, 4);
+      mbar_init(bars + Bar::s_full + 8 * i, 1);
+      mbar_init(bars + Bar::p_full + 8 * i, 4);
+      mbar_init(bars + Bar::pv_done + 8 * i, 1);
+    }
+    mbar_init(bars + Bar::drain, 1);
+    *abort_s = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(bars + Bar::tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  absent = __syncthreads_or(absent);
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::bars + Bar::tmem);
+  int fail = 0;
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+    if (warp == 12) {
+      // ---------------------------------------------------------------- MMA
+      constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);                     // 8-row groups, version, 128-byte swizzle
+      constexpr uint32_t idesc_s = idesc_f16(kN, false), idesc_o = idesc_f16(D, true);
+      const uint32_t q_lo = ((base + L::q) >> 4) | (1u << 16), k_lo = ((base + L::k) >> 4) | (1u << 16);
+      const uint32_t v_lo = ((base + L::v) >> 4) | ((uint32_t)(L::kHalf >> 4) << 16);     // leading offset: the next 64 channels
+      auto scores = [&](int t, int stage) {
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
+            mma_f16_ss(tmem + t * kN, q_lo + t * (L::kOperand >> 4) + off, k_lo + stage * (L::kOperand >> 4) + off, HI, idesc_s, kk > 0);
+          }
+          tc_commit(bars + Bar::s_full + 8 * t);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](int bar) {
+        if (elect_one()) tc_commit(bars + bar);
+        __syncwarp();
+      };
+      for (int t = 0; t < 2 && fail == 0; ++t)
+        if (R.count[t] > 0) fail = wait_bar<62>(bars + Bar::q_full + 8 * t, 0);
+      if (fail == 0 && steps > 0) {
+        fail = wait_bar<63>(bars + Bar::k_full, 0);
+        if (fail == 0) {
+          tc_fence_after();
+          for (int t = 0; t < 2; ++t)
+            if (R.count[t] > 0) scores(t, 0);
+          commit(Bar::k_empty);
+        }
+      }
+#pragma unroll 1
+      for (int j = 0; j < steps && fail == 0; ++j) {
+        const int stage = j & 1, next = stage ^ 1;
+        bool have_v = false, have_k = false;
+#pragma unroll 1
+        for (int t = 0; t < 2 && fail == 0; ++t) {
+          if (j >= R.count[t]) continue;
+          if (!have_v) fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1);
+          have_v = true;
+          if (fail == 0) fail = wait_bar<65>(bars + Bar::p_full + 8 * t, j & 1);
+          if (fail != 0) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kN / 16; ++kk)
+              mma_f16_ts(tmem + 256 + t * 128, tmem + t * kN + kk * 8, v_lo + stage * (L::kOperand >> 4) + kk * (2048 >> 4), HI, idesc_o, j > 0 || kk > 0);
+            tc_commit(bars + Bar::pv_done + 8 * t);
+          }
+          __syncwarp();
+          if (j + 1 < R.count[t]) {
+            if (!have_k) fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1);
+            have_k = true;
+            if (fail != 0) break;
+            tc_fence_after();
+            scores(t, next);
+          }
+        }
+        if (fail != 0) break;
+        commit(Bar::v_empty + 8 * stage);
+        if (have_k) commit(Bar::k_empty + 8 * next);
+      }
+      if (fail != 0) {
+        give_up(abort_s, P.status, fail);
+        commit(Bar::drain);
+        mbar_wait<true>(bars + Bar::drain, 0, 1u << 16);
+      }
+    }
+  } else if (warp >= 8) {
+    // ---------------------------------------------------------------- cache -> fp16 tiles: a warp 32 keys of each
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFillRegs));
+    const int w = warp - 8, n = lane >> 2, c = lane & 3;
+    const int64_t page_bytes = (int64_t)A.Hkv * (A.page_size / 16) * Rec::kBytes;
+    const uint8_t* const head = A.data + (int64_t)h * (A.page_size / 16) * Rec::kBytes;
+    const bool halves = A.page_size < 32;
+    int ids0 = -1, ids1 = -1;                                  // page ids of 32 tiles, one per lane
+    const uint8_t* rec[2] = {nullptr, nullptr};                // records of the tile whose loads come next; null: zeros
+    auto find = [&](int j) {
+      const int key = key_begin + j * kN + w * 32;
+      if ((j & 31) == 0) {
+        const int mine = key + lane * kN;
+        ids0 = mine < key_end ? __ldg(table + (mine >> P.page_shift)) : -1;
+        if (halves) ids1 = mine + 16 < key_end ? __ldg(table + ((mine + 16) >> P.page_shift)) : -1;
+      }
+      const int p0 = __shfl_sync(0xffffffffu, ids0, j & 31), p1 = halves ? __shfl_sync(0xffffffffu, ids1, j & 31) : p0;
+      const bool ok0 = (uint32_t)p0 < (uint64_t)A.num_pages, ok1 = (uint32_t)p1 < (uint64_t)A.num_pages && key + 16 < key_end;
+      const int in0 = (key & (A.page_size - 1)) >> 4;
+      rec[0] = ok0 ? head + p0 * page_bytes + in0 * Rec::kBytes : nullptr;
+      rec[1] = ok1 ? head + p1 * page_bytes + (halves ? 0 : in0 + 1) * Rec::kBytes : nullptr;
+    };
+    constexpr int W = D / 32;                                  // words of a lane's codes of a token (keys), of two tokens (values)
+    uint32_t kx[2][2][W], vx[2][2][W], ks[2], vs[2];
+    auto load = [&](const uint8_t* from, uint32_t (&x)[W]) {
+      if constexpr (D == 128) {
+        const uint4 u = from ? __ldg(reinterpret_cast<const uint4*>(from) + lane) : make_uint4(0, 0, 0, 0);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+      } else {
+        const uint2 u = from ? __ldg(reinterpret_cast<const uint2*>(from) + lane) : make_uint2(0, 0);
+        x[0] = u.x; x[1] = u.y;
+      }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        load(rec[r], kx[r][0]);
+        load(rec[r] ? rec[r] + 4 * D : nullptr, kx[r][1]);
+        ks[r] = vs[r] = 0;
+        if (rec[r]) {
+          if constexpr (D == 128) ks[r] = __ldg(reinterpret_cast<const uint32_t*>(rec[r] + Rec::kKeyScales) + lane);
+          else ks[r] = __ldg(reinterpret_cast<const uint16_t*>(rec[r] + Rec::kKeyScales) + lane);
+          vs[r] = __ldg(reinterpret_cast<const uint32_t*>(rec[r] + Rec::kValueScales) + (D == 128 ? lane : (lane >> 3) * 4 + c));
+        }
+      }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        load(rec[r] ? rec[r] + Rec::kValues : nullptr, vx[r][0]);
+        load(rec[r] ? rec[r] + Rec::kValues + 4 * D : nullptr, vx[r][1]);
+      }
+    };
+    if (steps > 0) {
+      find(0);
+      load_k();
+      load_v();
+    }
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+      const int stage = j & 1, key0 = key_begin + j * kN + w * 32;
+      const uint32_t sk = base + L::k + stage * L::kOperand, sv = base + L::v + stage * L::kOperand;
+      if (j >= 2 && (fail = wait_bar<60>(bars + Bar::k_empty + 8 * stage, ((j >> 1) - 1) & 1)) != 0) break;
+      uint32_t vsc[2] = {vs[0], vs[1]};
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        // values of keys that no row sees are zeros, whatever lies there
+        if (key0 + 16 * r + 16 > see_any) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key0 + 16 * r + 2 * c + (i & 1) + (i >> 1) * 8 >= see_any) vsc[r] &= ~(0xffu << (8 * i));
+        }
+        // A NaN scale of a value must not reach rows that do not see its key (0 times NaN): the key becomes NaN in its place, whose
+        // scores are masked in those rows, and the value 0.
+        bool poison[2] = {false, false};
+        if (__any_sync(0xffffffffu, (((vsc[r] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0)) {
+          uint32_t nan_keys[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool bad = (vsc[r] >> (8 * i) & 0x7fu) == 0x7fu;
+            nan_keys[i] = __ballot_sync(0xffffffffu, bad) & (0x11111111u << (n >> 1));
+            if (bad) vsc[r] &= ~(0xffu << (8 * i));
+          }
+          poison[0] = (n & 1 ? nan_keys[1] : nan_keys[0]) != 0;
+          poison[1] = (n & 1 ? nan_keys[3] : nan_keys[2]) != 0;
+        }
+        // Lanes 2 and 3 of a quad (D=128) take their words in another order, so that 8 lanes' stores meet different banks: those of rows
+        // n and n + 1 and channels 32 c ... fall on the same 128 bytes for c and c + 2.
+        const bool turn = D == 128 && c >= 2;
+        const uint32_t f0 = e4m3x2_to_f16(ks[r]), f1 = D == 128 ? e4m3x2_to_f16(ks[r] >> 16) : f0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                          // tokens n, n + 8
+          const int row = w * 32 + r * 16 + i * 8 + n;
+          uint32_t sc[2];
+          if constexpr (D == 128) {
+            sc[0] = splat(i ? f1 : f0, turn); sc[1] = splat(i ? f1 : f0, !turn);
+          } else {
+            sc[0] = sc[1] = splat(f0, i);
+          }
+          if (poison[i]) sc[0] = sc[1] = 0x7e007e00u;
+#pragma unroll
+          for (int x = 0; x < W; ++x) {
+            const uint32_t code = D == 128 ? (turn ? kx[r][i][x ^ 2] : kx[r][i][x]) : kx[r][i][x];
+            uint32_t y[4];
+            e2m1x8_to_f16(code, y);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) y[z] = hmul2(y[z], sc[D == 128 ? x >> 1 : 0]);
+            sts128(sk + L::at(row, c * W + (D == 128 && turn ? x ^ 2 : x)), y);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + Bar::k_full + 8 * stage);
+      const bool more = j + 1 < steps;
+      if (more) {
+        find(j + 1);
+        load_k();
+      }
+      if (j >= 2 && (fail = wait_bar<61>(bars + Bar::v_empty + 8 * stage, ((j >> 1) - 1) & 1)) != 0) break;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                          // tokens 2 c + 8 i and the next; odd n (D=128) the other way round
+          const uint32_t f = e4m3x2_to_f16(vsc[r] >> (16 * i));
+          const bool turn = D == 128 && (n & 1);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = w * 32 + r * 16 + i * 8 + 2 * c + (turn ? e ^ 1 : e);
+            const uint32_t sc = splat(f, turn ? e == 0 : e == 1);
+#pragma unroll
+            for (int x = 0; x < W / 2; ++x) {
+              const uint32_t code = turn ? vx[r][i][(e ^ 1) * (W / 2) + x] : vx[r][i][e * (W / 2) + x];
+              uint32_t y[4];
+              e2m1x8_to_f16(code, y);
+#pragma unroll
+              for (int z = 0; z < 4; ++z) y[z] = hmul2(y[z], sc);
+              sts128(sv + L::at(row, n * (W / 2) + x), y);
+            }
+          }
+        }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + Bar::v_full + 8 * stage);
+      if (more) load_v();
+    }
+    if (fail != 0) give_up(abort_s, P.status, fail);
+  } else {
+    // ---------------------------------------------------------------- softmax: thread r of the warpgroup has row r of its tile
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * kM + r, count = R.count[t];
+    const bool real = row < rows;
+    const int tok = real ? row / P.group : 0, hq = h * P.group + (real ? row - tok * P.group : 0);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tm_s = tmem + t * kN + lanes, tm_o = tmem + 256 + t * 128 + lanes;
+    float factor, add = 0.f;
+    {
+      const uint4* const src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.q + (int64_t)(seq.q0 + tok) * A.q_sn + hq * A.q_sh);
+      uint4 x[D / 8];
+      uint32_t m2 = 0;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (real && i * 8 < A.D) x[i] = __ldg(src + i);
+        m2 = habsmax2(m2, habsmax2(habsmax2(x[i].x, x[i].y), habsmax2(x[i].z, x[i].w)));
+      }
+      m2 = abs2(m2);
+      const RowScale scale(fmaxf(bf16_lo(m2), bf16_hi(m2)));
+      factor = fmaxf(scale.undo * P.scale_log2, 1.2e-38f);     // (never 0: it multiplies the -inf of masked scores)
+      if (A.lse != nullptr && A.k_offset != nullptr && split == 0 && real) {          // scores of the keys with their offset: scale q . offset more
+        const uint4* const off = reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.k_offset + (int64_t)h * A.D);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          if (i * 8 < A.D) {
+            const uint4 o = __ldg(off + i);
+            add = fmaf(bf16_lo(x[i].x), bf16_lo(o.x), fmaf(bf16_hi(x[i].x), bf16_hi(o.x), add));
+            add = fmaf(bf16_lo(x[i].y), bf16_lo(o.y), fmaf(bf16_hi(x[i].y), bf16_hi(o.y), add));
+            add = fmaf(bf16_lo(x[i].z), bf16_lo(o.z), fmaf(bf16_hi(x[i].z), bf16_hi(o.z), add));
+            add = fmaf(bf16_lo(x[i].w), bf16_lo(o.w), fmaf(bf16_hi(x[i].w), bf16_hi(o.w), add));
+          }
+        add *= A.sm_scale;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t y[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) y[z] = pack_f16(bf16_lo(u[z]) * scale.up, bf16_hi(u[z]) * scale.up);
+        sts128(base + L::q + t * L::kOperand + L::at(r, i), y);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + Bar::q_full + 8 * t);
+    }
+    const int limit = real ? seq.seen(A, tok) : 0x7fffffff;    // keys that the row sees
+    const int limit_all = __reduce_min_sync(0xffffffffu, limit);
+    float m = kLowest;
+    float2 l = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int j = 0; j < count; ++j) {
+      if ((fail = wait_bar<66>(bars + Bar::s_full + 8 * t, j & 1)) != 0) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, s[i]);
+      tmem_wait_ld();
+      const int key0 = key_begin + j * kN;
+      if (key0 + kN > limit_all) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (key0 + 32 * i + x >= limit) s[i][x] = 0xff800000u;
+      }
+      if (absent) {                        // some page of the item's keys is not in the cache (the whole CTA knows)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (key0 + 16 * i < key_end && !has_page(key0 + 16 * i)) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) s[i >> 1][(i & 1) * 16 + x] = 0xff800000u;
+          }
+      }
+      float top = kLowest, top2 = kLowest;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          top = fmaxf(top, fmaxf(__uint_as_float(s[i][x]), __uint_as_float(s[i][x + 1])));
+          top2 = fmaxf(top2, fmaxf(__uint_as_float(s[i][x + 2]), __uint_as_float(s[i][x + 3])));
+        }
+      top = fmaxf(top, top2) * factor;
+      if (__any_sync(0xffffffffu, top > m + kSlack)) {
+        const float m_new = fmaxf(m, top), corr = ex2_approx(m - m_new);
+        m = m_new;
+        l.x *= corr; l.y *= corr;
+        if (j > 0) {
+          if ((fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (j - 1) & 1)) != 0) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o[32];
+            tmem_ld32(tm_o + 32 * i, o);
+            tmem_wait_ld();
+            uint32_t o0[16], o1[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              o0[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+              o1[x] = __float_as_uint(__uint_as_float(o[16 + x]) * corr);
+            }
+            tmem_st16(tm_o + 32 * i, o0);
+            tmem_st16(tm_o + 32 * i + 16, o1);
+          }
+        }
+      }
+      const float2 f2 = make_float2(factor, factor), base2 = make_float2(kTop - m, kTop - m);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t p[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          float2 e = ffma2(make_float2(__uint_as_float(s[i][2 * x]), __uint_as_float(s[i][2 * x + 1])), f2, base2);
+          e.x = ex2_approx(e.x); e.y = ex2_approx(e.y);
+          l = fadd2(l, e);
+          p[x] = pack_f16(e.x, e.y);
+        }
+        tmem_st16(tm_s + 16 * i, p);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + Bar::p_full + 8 * t);
+    }
+    if (fail == 0 && count > 0) fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (count - 1) & 1);
+    if (fail != 0) {
+      give_up(abort_s, P.status, fail);
+    } else if (P.splits == 1 || count > 0) {
+      tc_fence_after();
+      const float sum = l.x + l.y, inv = sum == 0.f ? 0.f : 1.0f / sum;
+      const int64_t place = ((int64_t)bh * P.tiles + tile) * kItemRows + t * kM + r;
+      const int64_t part = (int64_t)split * heads * P.tiles * kItemRows + place;
+      __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh;
+#pragma unroll 1
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t o[32];
+        if (count > 0) {
+          tmem_ld32(tm_o + 32 * i, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0;
+        }
+        if (real) {
+          if (P.splits == 1) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 8)
+              if (32 * i + x < A.D) {
+                uint32_t y[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) y[z] = pack_bf16(__uint_as_float(o[x + 2 * z]) * inv, __uint_as_float(o[x + 2 * z + 1]) * inv);
+                *reinterpret_cast<uint4*>(out + 32 * i + x) = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<uint4*>(P.o_part + part * D + 32 * i + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+          }
+        }
+      }
+      if (real && P.splits > 1) P.ml_part[part] = make_float2(m, sum);
+      if (real && A.lse != nullptr) {
+        if (P.splits == 1) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, sum, add);
+        else if (split == 0) P.lse_add[place] = add;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The splits of a row joined: a warp per row, a lane D / 32 channels, in the order of the keys.
+template <int D>
+__global__ void __launch_bounds__(256) kv_prefill_join_kernel(const Params2 P) {
+  constexpr int V = D / 32;
+  const KvAttnArgs& A = P.a;
+  const int lane = threadIdx.x & 31;
+  const uint32_t id = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int in_tile = id % kItemRows, item = id / kItemRows, tile = item % P.tiles, bh = item / P.tiles;
+  if (bh >= A.B * A.Hkv) return;                                // (a whole warp; others of the CTA wait below)
+  const int b = bh / A.Hkv, h = bh - b * A.Hkv;
+  const KvSeq seq(A, b);
+  const int rows = seq.q_len * P.group, row = tile * kItemRows + in_tile;
+  pdl_wait();                              // also where there is no row: what follows on the stream may write the first kernel's inputs
+  if (row >= rows) return;
+  const Range R(seq, P, tile * kItemRows, rows, 0);
+  const int n = R.n[in_tile / kM], all = max(R.n[0], R.n[1]), per = (all + P.splits - 1) / P.splits;
+  const int used = n > 0 ? (n + per - 1) / per : 0;
+  const int64_t place = (int64_t)item * kItemRows + in_tile, step = (int64_t)A.B * A.Hkv * P.tiles * kItemRows;
+  float m = kLowest;
+  for (int s = lane; s < used; s += 32) m = fmaxf(m, P.ml_part[place + s * step].x);
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float acc[V], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < used; ++s) {
+    const int64_t at = place + s * step;
+    const float2 ml = P.ml_part[at];
+    const float w = ex2_approx(ml.x - m);
+    l = fmaf(w, ml.y, l);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(P.o_part + at * D + lane * V + i);
+      acc[i] = fmaf(w, v.x, acc[i]); acc[i + 1] = fmaf(w, v.y, acc[i + 1]);
+    }
+  }
+  const int tok = row / P.group, hq = h * P.group + row - tok * P.group;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh + lane * V;
+  if (lane * V < A.D) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16(acc[i] * inv, acc[i + 1] * inv);
+  }
+  if (lane == 0 && A.lse != nullptr) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, used > 0 ? P.lse_add[place] : 0.f);
+}
+
+inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct Plan2 {
+  int tiles, splits;
+  int64_t items;
+  size_t add, ml, o, bytes;               // offsets in the workspace
+};
+
+Plan2 plan2(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
+  Plan2 p;
+  p.tiles = (int)(((int64_t)max_q * (Hq / Hkv) + kItemRows - 1) / kItemRows);
+  p.items = (int64_t)B * Hkv * p.tiles;
+  const int64_t key_tiles = ((int64_t)max_k + kN - 1) / kN, room = sms / p.items, most = (key_tiles + 3) / 4;
+  p.splits = (int)(room < most ? room : most);
+  if (p.splits < 1) p.splits = 1;
+  const size_t rows = p.splits > 1 ? (size_t)p.items * kItemRows : 0;
+  p.add = 256;
+  p.ml = p.add + align256(rows * 4);
+  p.o = p.ml + align256(rows * p.splits * 8);
+  p.bytes = p.o + align256(rows * p.splits * DS * 4);
+  return p;
+}
+
+template <int D>
+cudaError_t launch(const Params2& P, const Plan2& p, cudaStream_t stream) {
+  constexpr int smem = Lay<D>::total + 1024;
+  // asked once: what the register hand-over relies on
+  static const cudaError_t regs_ok = [] {
+    cudaFuncAttributes f;
+    const cudaError_t e = cudaFuncGetAttributes(&f, kv_prefill_kernel<D>);
+    return e != cudaSuccess ? e : f.numRegs < kLaunchRegs ? cudaErrorInvalidConfiguration : cudaSuccess;
+  }();
+  if (regs_ok != cudaSuccess) return regs_ok;
+  if (cudaError_t e = cudaFuncSetAttribute(kv_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return e;
+  if (cudaError_t e = launch_pdl(kv_prefill_kernel<D>, dim3((unsigned)p.items, P.splits), kThreads2, smem, stream, false, P); e != cudaSuccess) return e;
+  if (P.splits == 1) return cudaGetLastError();
+  return launch_pdl(kv_prefill_join_kernel<D>, dim3((unsigned)(p.items * kItemRows / 8)), 256, 0, stream, true, P);
+}
+
+}  // namespace
+
+bool kv_prefill_takes(int Hq, int Hkv, int DS, int max_q, int max_k) { return (int64_t)max_q * (Hq / Hkv) > 64; }
+
+size_t kv_prefill_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) { return plan2(B, Hq, Hkv, DS, max_q, max_k, sms).bytes; }
+
+bool kv_prefill_fits(int B, int Hq, int Hkv, int max_q) {
+  const int64_t rows = (int64_t)max_q * (Hq / Hkv), tiles = (rows + kItemRows - 1) / kItemRows;
+  return (int64_t)B * Hkv * tiles * kItemRows < (1ll << 31);
+}
+
+cudaError_t launch_kv_prefill(const KvAttnArgs& a, cudaStream_t stream) {
+  int sms;
+  if (cudaError_t e = sm_count(&sms); e != cudaSuccess) return e;
+  const Plan2 p = plan2(a.B, a.Hq, a.Hkv, a.DS, a.max_q, a.max_k, sms);
+  Params2 P;
+  P.a = a;
+  P.group = a.Hq / a.Hkv; P.tiles = p.tiles; P.splits = p.splits;
+  P.scale_log2 = a.sm_scale * kLog2e;
+  P.page_shift = 0;
+  while ((1 << P.page_shift) < a.page_size) ++P.page_shift;
+  char* const w = (char*)a.workspace;
+  P.status = a.status != nullptr ? a.status : (int*)w;
+  P.lse_add = (float*)(w + p.add); P.ml_part = (float2*)(w + p.ml); P.o_part = (float*)(w + p.o);
+  return a.DS == 128 ? launch<128>(P, p, stream) : launch<64>(P, p, stream);
+}
+
+}  // namespace sage3

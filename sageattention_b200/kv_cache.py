@@ -383,7 +383,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache
 def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tensor, kv_lens: torch.Tensor,
                      cu_seqlens_q: Optional[torch.Tensor] = None, max_seqlen_q: int = 1, max_seqlen_k: Optional[int] = None,
                      is_causal: bool = True, sm_scale: Optional[float] = None, return_lse: bool = False,
-                     out: Optional[torch.Tensor] = None):
+                     out: Optional[torch.Tensor] = None, check_status: bool = False):
     """Attention of new tokens over the 4-bit cache, their own keys (already appended) among the last ones.
 
     q: bf16 ``[tokens, Hq, head_dim]``, ``Hq`` a multiple of the cache's heads; sequence i has rows ``cu_seqlens_q[i] ... cu_seqlens_q[i+1]`` (int32
@@ -395,7 +395,7 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     Attention is over the values that the cache stands for, queries and softmax are not quantised.  Rows that see no key give zeros and an
     LSE of ``-inf``; keys of pages outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not
     touched in ``out`` (or are undefined in a new tensor).  Returns the output like q, and with ``return_lse`` the natural-log LSE fp32
-    ``[tokens, Hq]`` of ``sm_scale * q.k``."""
+    ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where one of their bounded waits gave up."""
     if out is not None:
         _check_out(out, q)
     key = ("kvcache", _sig(q), cache._key, _sig(block_table), _sig(kv_lens), _sig(cu_seqlens_q), max_seqlen_q, max_seqlen_k, bool(is_causal), sm_scale)
@@ -417,7 +417,13 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
         if cu_seqlens_q is not None:
             a.cu_seqlens_q = cu_seqlens_q.data_ptr()
         a.workspace = ws.data_ptr()
+        status = torch.empty(1, dtype=torch.int32, device=dev) if check_status else None
+        if status is not None:
+            a.device_status = status.data_ptr()
         _run(_lib.load().sage3_kv_attention, a, dev, "sage3_kv_attention")
+        if status is not None:
+            with _on_device(dev):
+                _lib.check(_lib.load().sage3_read_device_status(status.data_ptr(), _stream_ptr(dev), None), "attention kernel")
     return (out, lse) if return_lse else out
 
 

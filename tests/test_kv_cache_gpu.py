@@ -264,7 +264,7 @@ def check(q, cache, table, kv_lens, q_lens, **kw):
     cu = np.concatenate(([0], np.cumsum(q_lens)))
     plain = kw.pop("no_cu", False)
     args = dict(max_seqlen_q=max(q_lens)) if not plain else {}
-    out, lse = sa.sageattn_kvcache(q, cache, table.to(DEV), torch.tensor(kv_lens, **i32), None if plain else torch.tensor(cu, **i32), return_lse=True,
+    out, lse = sa.sageattn_kvcache(q, cache, table.to(DEV), torch.tensor(kv_lens, **i32), None if plain else torch.tensor(cu, **i32), return_lse=True, check_status=True,
                                    is_causal=kw.get("causal", True), sm_scale=kw.get("scale"), **args)
     alone = sa.sageattn_kvcache(q, cache, table.to(DEV), torch.tensor(kv_lens, **i32), None if plain else torch.tensor(cu, **i32),
                                 is_causal=kw.get("causal", True), sm_scale=kw.get("scale"), **args)
