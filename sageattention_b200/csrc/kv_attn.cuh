@@ -7,8 +7,8 @@
 namespace sage3 {
 
 // The running maximum of a row need not be its maximum: weights are 2^(s - m + kTop), and m is brought up to date only where a score
-// passes it by more than kSlack.  Weights stay below 2^15, within fp16, and those of 2^-22 of the largest keep all their bits.
-constexpr float kTop = 8.f, kSlack = 7.f;
+// passes it by more than kSlack.  Weights stay below 2^15, within fp16, and those of 2^-20 of the largest keep all their bits.
+constexpr float kTop = 6.f, kSlack = 9.f;
 constexpr float kLowest = -1e38f;         // the maximum of a row that has seen no key
 
 // Where a sequence's rows and keys lie; every bound that memory accesses rely on is taken here.

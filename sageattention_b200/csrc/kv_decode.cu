@@ -53,27 +53,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t splat_lo(uint32_t x) { return __byte_perm(x, 0, 0x1010); }
 __device__ __forceinline__ uint32_t splat_hi(uint32_t x) { return __byte_perm(x, 0, 0x3232); }
-__device__ __forceinline__ uint4 lds128(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at));
-  return v;
-}
-
 // 128-key blocks of an item (one at least, so that rows without keys are written too) and items per kv head
 __device__ __forceinline__ int blocks_of(const KvSeq& s) { return max(1, (s.kv_len + kBlock - 1) / kBlock); }
 template <int kRows>

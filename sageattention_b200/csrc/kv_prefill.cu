@@ -1,13 +1,16 @@
 // Attention of many query rows per kv head over the 4-bit cache: chunks of prompts behind cached prefixes.
 //
 // A CTA takes 256 rows (tokens times the heads of a kv head, two tiles of 128) of a (sequence, kv head) and walks tiles of 128 keys:
-//   warps 8-11   read records of the cache as they are, turn codes and scales into fp16 (exact, see kv_decode.cu) and write K and V tiles
-//                to shared memory, once for all 256 rows.  Both lie alike, rows of keys with 128-byte swizzle: K is then the K-major B
-//                operand of S = Q K^T and V the MN-major one of O += P V, so nothing is transposed
-//   warp  12     issues the tcgen05.mma kind::f16: S_t = Q_t K^T (queries from shared memory), O_t += P_t V (P from tensor memory)
+//   warps 8-11   fetch the keys' part of the records as it is, turn codes and scales into fp16 (exact, see kv_decode.cu) and write K
+//                tiles to shared memory, once for all 256 rows
+//   warps 12-15  the same with values.  Both tiles lie alike, rows of keys with 128-byte swizzle: K is then the K-major B operand of
+//                S = Q K^T and V the MN-major one of O += P V, so nothing is transposed
+//   warp  16     issues the tcgen05.mma kind::f16: S_t = Q_t K^T (queries from shared memory), O_t += P_t V (P from tensor memory)
 //   warps 0-3    softmax of row tile 0, a thread per row: scores from tensor memory to registers, weights back over them in fp16
 //   warps 4-7    the same for row tile 1; one tile's softmax runs beside the other's MMAs
-// A row's maximum is brought up to date only where a score passes it by 2^7 (kv_attn.cuh); then its thread rescales the row of O.
+// A row's maximum need not be its maximum (kv_attn.cuh): a thread takes the weights of 64 keys against the one that it has, and only where
+// their sum shows one too large for fp16 does it look for the maximum, rescale its row of O and take them again.  The P V of the
+// first 64 keys of a tile runs beside the softmax of the others.
 // With few items the keys are split over CTAs as well and joined by a second kernel.
 //
 // Tensor memory (512 columns): S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t takes the first 64 columns of S_t:
@@ -15,27 +18,35 @@
 //
 // Every wait on an mbarrier is bounded; where one gives up the CTA records its code in *status, waits (bounded) for its MMAs in
 // flight, frees its tensor memory and returns: 60 K stage free, 61 V stage free, 62 Q there, 63 K there, 64 V there, 65 P there, 66 scores
-// there, 67 last P V done.
+// there, 67 last P V done; 68 tensor memory begins elsewhere.
 #include "kv_attn.cuh"
 
 namespace sage3 {
 
 namespace {
 
-constexpr int kThreads2 = 512, kM = 128, kN = 128, kItemRows = 2 * kM;
-// Register hand-over (setmaxnreg) moves registers inside the pool the CTA was launched with, 128 a thread; launch() checks that.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kFillRegs = 80, kRoleRegs = 48;
-static_assert(256 * kSoftmaxRegs + 128 * (kFillRegs + kRoleRegs) <= kThreads2 * kLaunchRegs, "setmaxnreg split exceeds the CTA's register pool");
+constexpr int kThreads2 = 640, kM = 128, kN = 128, kItemRows = 2 * kM;
+// Register hand-over (setmaxnreg) moves registers inside the pool the CTA was launched with, 96 a thread; launch() checks that.
+constexpr int kLaunchRegs = 96, kSoftmaxRegs = 136, kFillRegs = 72, kRoleRegs = 56;
+static_assert(256 * kSoftmaxRegs + 256 * kFillRegs + 128 * kRoleRegs <= kThreads2 * kLaunchRegs, "setmaxnreg split exceeds the CTA's register pool");
+
+template <int v>
+struct Int {
+  static constexpr int value = v;
+};
 
 template <int D>
 struct Lay {                              // shared memory
   static constexpr int kOperand = kM * D * 2, kHalf = kM * 128;      // a tile; its part of 64 channels
-  static constexpr int q = 0, k = 2 * kOperand, v = 4 * kOperand, bars = 6 * kOperand, total = bars + 256;
+  static constexpr int q = 0, k = 2 * kOperand, v = 4 * kOperand;
+  // parts of a tile's records as they are, two per warp: keys with both kinds of scales, and values with theirs
+  static constexpr int kKeyPart = 10 * D, kValuePart = 9 * D, raw_k = 6 * kOperand, raw_v = raw_k + 8 * kKeyPart, kRaw = 8 * (kKeyPart + kValuePart), raw = raw_k;
+  static constexpr int bars = raw + kRaw, total = bars + 256;
   // 16 bytes: channels 8 chunk ... of a row
   static __device__ __forceinline__ int at(int row, int chunk) { return (chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 };
-struct Bar {                              // byte offsets in the barrier block, two of each
-  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96, pv_done = 112, drain = 128, tmem = 144, abort = 152;
+struct Bar {                              // byte offsets in the barrier block, of two each but for p_full and the last
+  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96 /* [half][tile] */, pv_half = 128, pv_done = 144, drain = 160, tmem = 176, abort = 184;
 };
 
 struct Params2 {
@@ -77,10 +88,46 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo
 __device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&x)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
 }
+__device__ __forceinline__ void lds(uint32_t at, uint32_t (&x)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
+}
+__device__ __forceinline__ void lds(uint32_t at, uint32_t (&x)[2]) { asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at)); }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr) : "memory");
+}
+// Waits for the tensor-memory loads under way; names the registers, so that nothing that reads them can be moved in front of it.
+__device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :: "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+}
 __device__ __forceinline__ uint32_t splat(uint32_t pair, bool hi) { return __byte_perm(pair, 0, hi ? 0x3232 : 0x1010); }
 
 // fp16 x fp16 -> fp32, A K-major, B K-major or (transposed) MN-major
 __host__ __device__ constexpr uint32_t idesc_f16(int N, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kM >> 4) << 24); }
+
+// What the scales of a lane's values (block n, tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of a record of which `seen` keys are seen by any row)
+// are replaced by, and whether keys n (bit 0) and n + 8 (bit 1) are to become NaN.  Values of keys that no row sees are zeros, whatever
+// lies there.  A NaN scale of a value must not reach rows that do not see its key (0 times NaN): the key becomes NaN in its place,
+// whose scores are masked in those rows, and the value 0.
+__device__ __noinline__ uint2 mend_scales(uint32_t scales, int seen) {
+  const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
+  uint32_t nan_keys[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (2 * c + (i & 1) + (i >> 1) * 8 >= seen) scales &= ~(0xffu << (8 * i));
+    const bool bad = (scales >> (8 * i) & 0x7fu) == 0x7fu;
+    nan_keys[i] = __ballot_sync(0xffffffffu, bad) & (0x11111111u << (n >> 1));
+    if (bad) scales &= ~(0xffu << (8 * i));
+  }
+  return make_uint2(scales, ((n & 1 ? nan_keys[1] : nan_keys[0]) != 0 ? 1u : 0u) | ((n & 1 ? nan_keys[3] : nan_keys[2]) != 0 ? 2u : 0u));
+}
 
 template <int D>
 __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 P) {
@@ -120,13 +167,15 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       mbar_init(bars + Bar::q_full + 8 * i, 4);
       mbar_init(bars + Bar::s_full + 8 * i, 1);
       mbar_init(bars + Bar::p_full + 8 * i, 4);
+      mbar_init(bars + Bar::p_full + 16 + 8 * i, 4);
+      mbar_init(bars + Bar::pv_half + 8 * i, 1);
       mbar_init(bars + Bar::pv_done + 8 * i, 1);
+      mbar_init(bars + Bar::drain + 8 * i, 1);
     }
-    mbar_init(bars + Bar::drain, 1);
     *abort_s = 0;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(bars + Bar::tmem, 512);
     tmem_relinquish();
   }
@@ -136,20 +185,22 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::bars + Bar::tmem);
   int fail = 0;
 
-  if (warp >= 12) {
+  if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
-    if (warp == 12) {
+    if (warp == 16) {
       // ---------------------------------------------------------------- MMA
       constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);                     // 8-row groups, version, 128-byte swizzle
       constexpr uint32_t idesc_s = idesc_f16(kN, false), idesc_o = idesc_f16(D, true);
       const uint32_t q_lo = ((base + L::q) >> 4) | (1u << 16), k_lo = ((base + L::k) >> 4) | (1u << 16);
       const uint32_t v_lo = ((base + L::v) >> 4) | ((uint32_t)(L::kHalf >> 4) << 16);     // leading offset: the next 64 channels
-      auto scores = [&](int t, int stage) {
+      // (tensor memory begins at 0, all of it being this CTA's, and stages and tiles are unrolled: addresses are constants)
+      auto scores = [&](auto t_, auto stage_) {
+        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
-            mma_f16_ss(tmem + t * kN, q_lo + t * (L::kOperand >> 4) + off, k_lo + stage * (L::kOperand >> 4) + off, HI, idesc_s, kk > 0);
+            mma_f16_ss(t * kN, q_lo + t * (L::kOperand >> 4) + off, k_lo + stage * (L::kOperand >> 4) + off, HI, idesc_s, kk > 0);
           }
           tc_commit(bars + Bar::s_full + 8 * t);
         }
@@ -159,47 +210,55 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
         if (elect_one()) tc_commit(bars + bar);
         __syncwarp();
       };
-      for (int t = 0; t < 2 && fail == 0; ++t)
-        if (R.count[t] > 0) fail = wait_bar<62>(bars + Bar::q_full + 8 * t, 0);
+      const int count0 = R.count[0], count1 = R.count[1];
+      if (tmem != 0) fail = 68;
+      if (fail == 0 && count0 > 0) fail = wait_bar<62>(bars + Bar::q_full, 0);
+      if (fail == 0 && count1 > 0) fail = wait_bar<62>(bars + Bar::q_full + 8, 0);
       if (fail == 0 && steps > 0) {
         fail = wait_bar<63>(bars + Bar::k_full, 0);
         if (fail == 0) {
           tc_fence_after();
-          for (int t = 0; t < 2; ++t)
-            if (R.count[t] > 0) scores(t, 0);
+          if (count0 > 0) scores(Int<0>{}, Int<0>{});
+          if (count1 > 0) scores(Int<1>{}, Int<0>{});
           commit(Bar::k_empty);
         }
       }
-#pragma unroll 1
-      for (int j = 0; j < steps && fail == 0; ++j) {
-        const int stage = j & 1, next = stage ^ 1;
-        bool have_v = false, have_k = false;
-#pragma unroll 1
-        for (int t = 0; t < 2 && fail == 0; ++t) {
-          if (j >= R.count[t]) continue;
-          if (!have_v) fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1);
-          have_v = true;
-          if (fail == 0) fail = wait_bar<65>(bars + Bar::p_full + 8 * t, j & 1);
-          if (fail != 0) break;
+      auto tile = [&](auto t_, auto stage_, int j, int count, bool& have_v, bool& have_k) {
+        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value, next = stage ^ 1;
+        if (fail != 0 || j >= count) return;
+        if (!have_v && (fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1)) != 0) return;
+        have_v = true;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if ((fail = wait_bar<65>(bars + Bar::p_full + 16 * half + 8 * t, j & 1)) != 0) return;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kN / 16; ++kk)
-              mma_f16_ts(tmem + 256 + t * 128, tmem + t * kN + kk * 8, v_lo + stage * (L::kOperand >> 4) + kk * (2048 >> 4), HI, idesc_o, j > 0 || kk > 0);
-            tc_commit(bars + Bar::pv_done + 8 * t);
+            for (int kk = half * (kN / 32); kk < (half + 1) * (kN / 32); ++kk)
+              mma_f16_ts(256 + t * 128, t * kN + kk * 8, v_lo + stage * (L::kOperand >> 4) + kk * (2048 >> 4), HI, idesc_o, kk > 0 ? 1u : j > 0);
+            tc_commit(bars + (half ? Bar::pv_done : Bar::pv_half) + 8 * t);
           }
           __syncwarp();
-          if (j + 1 < R.count[t]) {
-            if (!have_k) fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1);
-            have_k = true;
-            if (fail != 0) break;
-            tc_fence_after();
-            scores(t, next);
-          }
         }
-        if (fail != 0) break;
+        if (j + 1 >= count) return;
+        if (!have_k && (fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1)) != 0) return;
+        have_k = true;
+        tc_fence_after();
+        scores(t_, Int<next>{});
+      };
+      auto step = [&](auto stage_, int j) {
+        constexpr int stage = decltype(stage_)::value;
+        bool have_v = false, have_k = false;
+        tile(Int<0>{}, stage_, j, count0, have_v, have_k);
+        tile(Int<1>{}, stage_, j, count1, have_v, have_k);
+        if (fail != 0) return;
         commit(Bar::v_empty + 8 * stage);
-        if (have_k) commit(Bar::k_empty + 8 * next);
+        if (have_k) commit(Bar::k_empty + 8 * (stage ^ 1));
+      };
+#pragma unroll 1
+      for (int j = 0; j < steps && fail == 0; j += 2) {
+        step(Int<0>{}, j);
+        if (j + 1 < steps && fail == 0) step(Int<1>{}, j + 1);
       }
       if (fail != 0) {
         give_up(abort_s, P.status, fail);
@@ -210,13 +269,16 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- cache -> fp16 tiles: a warp 32 keys of each
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFillRegs));
-    const int w = warp - 8, n = lane >> 2, c = lane & 3;
+    const bool keys = warp < 12;
+    const int w = warp & 3, n = lane >> 2, c = lane & 3;
     const int64_t page_bytes = (int64_t)A.Hkv * (A.page_size / 16) * Rec::kBytes;
     const uint8_t* const head = A.data + (int64_t)h * (A.page_size / 16) * Rec::kBytes;
     const bool halves = A.page_size < 32;
     int ids0 = -1, ids1 = -1;                                  // page ids of 32 tiles, one per lane
-    const uint8_t* rec[2] = {nullptr, nullptr};                // records of the tile whose loads come next; null: zeros
-    auto find = [&](int j) {
+    const int part = keys ? L::kKeyPart : L::kValuePart;
+    const uint32_t raw_at = base + (keys ? L::raw_k : L::raw_v) + 2 * w * part;
+    // this warp's part of two records of tile j on its way to the raw buffer; zeros where there is no page or no key that is seen
+    auto fetch = [&](int j) {
       const int key = key_begin + j * kN + w * 32;
       if ((j & 31) == 0) {
         const int mine = key + lane * kN;
@@ -225,134 +287,104 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       }
       const int p0 = __shfl_sync(0xffffffffu, ids0, j & 31), p1 = halves ? __shfl_sync(0xffffffffu, ids1, j & 31) : p0;
       const bool ok0 = (uint32_t)p0 < (uint64_t)A.num_pages, ok1 = (uint32_t)p1 < (uint64_t)A.num_pages && key + 16 < key_end;
-      const int in0 = (key & (A.page_size - 1)) >> 4;
-      rec[0] = ok0 ? head + p0 * page_bytes + in0 * Rec::kBytes : nullptr;
-      rec[1] = ok1 ? head + p1 * page_bytes + (halves ? 0 : in0 + 1) * Rec::kBytes : nullptr;
-    };
-    constexpr int W = D / 32;                                  // words of a lane's codes of a token (keys), of two tokens (values)
-    uint32_t kx[2][2][W], vx[2][2][W], ks[2], vs[2];
-    auto load = [&](const uint8_t* from, uint32_t (&x)[W]) {
-      if constexpr (D == 128) {
-        const uint4 u = from ? __ldg(reinterpret_cast<const uint4*>(from) + lane) : make_uint4(0, 0, 0, 0);
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-      } else {
-        const uint2 u = from ? __ldg(reinterpret_cast<const uint2*>(from) + lane) : make_uint2(0, 0);
-        x[0] = u.x; x[1] = u.y;
-      }
-    };
-    auto load_k = [&]() {
+      const uint8_t* const r0 = head + (ok0 ? p0 * page_bytes + ((key & (A.page_size - 1)) >> 4) * Rec::kBytes : 0);
+      const uint8_t* const r1 = halves ? head + (ok1 ? p1 * page_bytes : 0) : r0 + (ok1 ? Rec::kBytes : 0);
+      constexpr int kMost = 2 * L::kKeyPart;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        load(rec[r], kx[r][0]);
-        load(rec[r] ? rec[r] + 4 * D : nullptr, kx[r][1]);
-        ks[r] = vs[r] = 0;
-        if (rec[r]) {
-          if constexpr (D == 128) ks[r] = __ldg(reinterpret_cast<const uint32_t*>(rec[r] + Rec::kKeyScales) + lane);
-          else ks[r] = __ldg(reinterpret_cast<const uint16_t*>(rec[r] + Rec::kKeyScales) + lane);
-          vs[r] = __ldg(reinterpret_cast<const uint32_t*>(rec[r] + Rec::kValueScales) + (D == 128 ? lane : (lane >> 3) * 4 + c));
+      for (int x = 0; x < kMost; x += 512) {
+        const int at = x + lane * 16;
+        if (at < 2 * part) {
+          const bool second = at >= part, ok = second ? ok1 : ok0;
+          const int in = second ? at - part : at;
+          const int off = keys ? (in < Rec::kValues ? in : in + (Rec::kValueScales - Rec::kValues)) : in + Rec::kValues;
+          cp_async16(raw_at + at, ok ? (second ? r1 : r0) + off : head, ok);
         }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto load_v = [&]() {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        load(rec[r] ? rec[r] + Rec::kValues : nullptr, vx[r][0]);
-        load(rec[r] ? rec[r] + Rec::kValues + 4 * D : nullptr, vx[r][1]);
-      }
-    };
-    if (steps > 0) {
-      find(0);
-      load_k();
-      load_v();
-    }
+    constexpr int W = D / 32;                                  // words of a lane's codes of a token (keys), of two tokens (values)
+    const uint32_t scales_at = D == 128 ? lane * 4 : (lane >> 3) * 16 + c * 4;
+    if (steps > 0) fetch(0);
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
       const int stage = j & 1, key0 = key_begin + j * kN + w * 32;
-      const uint32_t sk = base + L::k + stage * L::kOperand, sv = base + L::v + stage * L::kOperand;
-      if (j >= 2 && (fail = wait_bar<60>(bars + Bar::k_empty + 8 * stage, ((j >> 1) - 1) & 1)) != 0) break;
-      uint32_t vsc[2] = {vs[0], vs[1]};
+      // all of it to registers, and the next on its way
+      cp_async_wait_all();
+      __syncwarp();
+      uint32_t x[2][2][W], ks[2] = {0, 0}, vsc[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        // values of keys that no row sees are zeros, whatever lies there
-        if (key0 + 16 * r + 16 > see_any) {
+        const uint32_t rec = raw_at + r * part;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (key0 + 16 * r + 2 * c + (i & 1) + (i >> 1) * 8 >= see_any) vsc[r] &= ~(0xffu << (8 * i));
-        }
-        // A NaN scale of a value must not reach rows that do not see its key (0 times NaN): the key becomes NaN in its place, whose
-        // scores are masked in those rows, and the value 0.
-        bool poison[2] = {false, false};
-        if (__any_sync(0xffffffffu, (((vsc[r] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0)) {
-          uint32_t nan_keys[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool bad = (vsc[r] >> (8 * i) & 0x7fu) == 0x7fu;
-            nan_keys[i] = __ballot_sync(0xffffffffu, bad) & (0x11111111u << (n >> 1));
-            if (bad) vsc[r] &= ~(0xffu << (8 * i));
-          }
-          poison[0] = (n & 1 ? nan_keys[1] : nan_keys[0]) != 0;
-          poison[1] = (n & 1 ? nan_keys[3] : nan_keys[2]) != 0;
-        }
-        // Lanes 2 and 3 of a quad (D=128) take their words in another order, so that 8 lanes' stores meet different banks: those of rows
-        // n and n + 1 and channels 32 c ... fall on the same 128 bytes for c and c + 2.
-        const bool turn = D == 128 && c >= 2;
-        const uint32_t f0 = e4m3x2_to_f16(ks[r]), f1 = D == 128 ? e4m3x2_to_f16(ks[r] >> 16) : f0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {                          // tokens n, n + 8
-          const int row = w * 32 + r * 16 + i * 8 + n;
-          uint32_t sc[2];
-          if constexpr (D == 128) {
-            sc[0] = splat(i ? f1 : f0, turn); sc[1] = splat(i ? f1 : f0, !turn);
-          } else {
-            sc[0] = sc[1] = splat(f0, i);
-          }
-          if (poison[i]) sc[0] = sc[1] = 0x7e007e00u;
-#pragma unroll
-          for (int x = 0; x < W; ++x) {
-            const uint32_t code = D == 128 ? (turn ? kx[r][i][x ^ 2] : kx[r][i][x]) : kx[r][i][x];
-            uint32_t y[4];
-            e2m1x8_to_f16(code, y);
-#pragma unroll
-            for (int z = 0; z < 4; ++z) y[z] = hmul2(y[z], sc[D == 128 ? x >> 1 : 0]);
-            sts128(sk + L::at(row, c * W + (D == 128 && turn ? x ^ 2 : x)), y);
-          }
-        }
+        for (int i = 0; i < 2; ++i) lds(rec + i * 4 * D + lane * 4 * W, x[r][i]);
+        vsc[r] = lds32(rec + (keys ? Rec::kValues : Rec::kValueScales - Rec::kValues) + scales_at);
+        if (keys) ks[r] = D == 128 ? lds32(rec + Rec::kKeyScales + lane * 4) : lds16(rec + Rec::kKeyScales + lane * 2);
       }
-      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars + Bar::k_full + 8 * stage);
-      const bool more = j + 1 < steps;
-      if (more) {
-        find(j + 1);
-        load_k();
+      if (j + 1 < steps) fetch(j + 1);
+      if (j >= 2) {
+        fail = keys ? wait_bar<60>(bars + Bar::k_empty + 8 * stage, ((j >> 1) - 1) & 1) : wait_bar<61>(bars + Bar::v_empty + 8 * stage, ((j >> 1) - 1) & 1);
+        if (fail != 0) break;
       }
-      if (j >= 2 && (fail = wait_bar<61>(bars + Bar::v_empty + 8 * stage, ((j >> 1) - 1) & 1)) != 0) break;
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r) {
+        uint32_t poison = 0;
+        if (key0 + 16 * r + 16 > see_any || __any_sync(0xffffffffu, (((vsc[r] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0)) {
+          const uint2 u = mend_scales(vsc[r], see_any - key0 - 16 * r);
+          vsc[r] = u.x; poison = u.y;
+        }
+        if (keys) {
+          // Lanes 2 and 3 of a quad (D=128) take their words in another order, so that 8 lanes' stores meet different banks: those of
+          // rows n and n + 1 and channels 32 c ... fall on the same 128 bytes for c and c + 2.
+          const bool turn = D == 128 && c >= 2;
+          const uint32_t sk = base + L::k + stage * L::kOperand;
+          const uint32_t f0 = e4m3x2_to_f16(ks[r]), f1 = D == 128 ? e4m3x2_to_f16(ks[r] >> 16) : f0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {                          // tokens 2 c + 8 i and the next; odd n (D=128) the other way round
-          const uint32_t f = e4m3x2_to_f16(vsc[r] >> (16 * i));
-          const bool turn = D == 128 && (n & 1);
+          for (int i = 0; i < 2; ++i) {                        // tokens n, n + 8
+            const int row = w * 32 + r * 16 + i * 8 + n;
+            uint32_t sc[2];
+            if constexpr (D == 128) {
+              sc[0] = splat(i ? f1 : f0, turn); sc[1] = splat(i ? f1 : f0, !turn);
+            } else {
+              sc[0] = sc[1] = splat(f0, i);
+            }
+            if (poison >> i & 1) sc[0] = sc[1] = 0x7e007e00u;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = w * 32 + r * 16 + i * 8 + 2 * c + (turn ? e ^ 1 : e);
-            const uint32_t sc = splat(f, turn ? e == 0 : e == 1);
-#pragma unroll
-            for (int x = 0; x < W / 2; ++x) {
-              const uint32_t code = turn ? vx[r][i][(e ^ 1) * (W / 2) + x] : vx[r][i][e * (W / 2) + x];
+            for (int z = 0; z < W; ++z) {
               uint32_t y[4];
-              e2m1x8_to_f16(code, y);
+              e2m1x8_to_f16(D == 128 && turn ? x[r][i][z ^ 2] : x[r][i][z], y);
 #pragma unroll
-              for (int z = 0; z < 4; ++z) y[z] = hmul2(y[z], sc);
-              sts128(sv + L::at(row, n * (W / 2) + x), y);
+              for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc[D == 128 ? z >> 1 : 0]);
+              sts128(sk + L::at(row, c * W + (D == 128 && turn ? z ^ 2 : z)), y);
+            }
+          }
+        } else {
+          const uint32_t sv = base + L::v + stage * L::kOperand;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {                        // tokens 2 c + 8 i and the next; odd n (D=128) the other way round
+            const uint32_t f = e4m3x2_to_f16(vsc[r] >> (16 * i));
+            const bool turn = D == 128 && (n & 1);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = w * 32 + r * 16 + i * 8 + 2 * c + (turn ? e ^ 1 : e);
+              const uint32_t sc = splat(f, turn ? e == 0 : e == 1);
+#pragma unroll
+              for (int z = 0; z < W / 2; ++z) {
+                uint32_t y[4];
+                e2m1x8_to_f16(turn ? x[r][i][(e ^ 1) * (W / 2) + z] : x[r][i][e * (W / 2) + z], y);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc);
+                sts128(sv + L::at(row, n * (W / 2) + z), y);
+              }
             }
           }
         }
+      }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars + Bar::v_full + 8 * stage);
-      if (more) load_v();
+      if (lane == 0) mbar_arrive(bars + (keys ? Bar::k_full : Bar::v_full) + 8 * stage);
     }
+    cp_async_wait_all();
     if (fail != 0) give_up(abort_s, P.status, fail);
   } else {
     // ---------------------------------------------------------------- softmax: thread r of the warpgroup has row r of its tile
@@ -405,80 +437,105 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
     const int limit_all = __reduce_min_sync(0xffffffffu, limit);
     float m = kLowest;
     float2 l = make_float2(0.f, 0.f);
-#pragma unroll 1
-    for (int j = 0; j < count; ++j) {
-      if ((fail = wait_bar<66>(bars + Bar::s_full + 8 * t, j & 1)) != 0) break;
+    // One key tile.  Scores come by 32 columns, the next ones on their way while these are worked on.  Masks and what else is rare stay out
+    // of the loop that nearly all tiles take: as one loop with branches it took a third longer, its code being fetched rather
+    // than run.
+    auto key_tile = [&](auto masked_, int j) {
+      constexpr bool masked = decltype(masked_)::value != 0;
+      if ((fail = wait_bar<66>(bars + Bar::s_full + 8 * t, j & 1)) != 0) return;
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, s[i]);
-      tmem_wait_ld();
       const int key0 = key_begin + j * kN;
-      if (key0 + kN > limit_all) {
+      auto mask = [&](int i, uint32_t (&s)[32]) {              // 32 scores from key 32 i of the tile on
+        const int key = key0 + 32 * i;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int x = 0; x < 32; ++x)
+          if (key + x >= limit) s[x] = 0xff800000u;
+        if (absent) {                      // some page of the item's keys is not in the cache (the whole CTA knows)
 #pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (key0 + 32 * i + x >= limit) s[i][x] = 0xff800000u;
-      }
-      if (absent) {                        // some page of the item's keys is not in the cache (the whole CTA knows)
+          for (int y = 0; y < 2; ++y)
+            if (key + 16 * y < key_end && !has_page(key + 16 * y)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (key0 + 16 * i < key_end && !has_page(key0 + 16 * i)) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) s[i >> 1][(i & 1) * 16 + x] = 0xff800000u;
-          }
-      }
-      float top = kLowest, top2 = kLowest;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          top = fmaxf(top, fmaxf(__uint_as_float(s[i][x]), __uint_as_float(s[i][x + 1])));
-          top2 = fmaxf(top2, fmaxf(__uint_as_float(s[i][x + 2]), __uint_as_float(s[i][x + 3])));
-        }
-      top = fmaxf(top, top2) * factor;
-      if (__any_sync(0xffffffffu, top > m + kSlack)) {
-        const float m_new = fmaxf(m, top), corr = ex2_approx(m - m_new);
-        m = m_new;
-        l.x *= corr; l.y *= corr;
-        if (j > 0) {
-          if ((fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (j - 1) & 1)) != 0) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t o[32];
-            tmem_ld32(tm_o + 32 * i, o);
-            tmem_wait_ld();
-            uint32_t o0[16], o1[16];
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              o0[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
-              o1[x] = __float_as_uint(__uint_as_float(o[16 + x]) * corr);
+              for (int x = 0; x < 16; ++x) s[16 * y + x] = 0xff800000u;
             }
-            tmem_st16(tm_o + 32 * i, o0);
-            tmem_st16(tm_o + 32 * i + 16, o1);
+        }
+      };
+      uint32_t s0[32], s1[32];
+      tmem_ld32(tm_s, s0);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[2][16];
+        float2 sum[2];
+        auto weights = [&](const uint32_t (&s)[32], uint32_t (&w)[16]) {
+          const float2 f2 = make_float2(factor, factor), base2 = make_float2(kTop - m, kTop - m);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            float2 e = ffma2(make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), f2, base2);
+            e.x = ex2_approx(e.x); e.y = ex2_approx(e.y);
+            sum[x & 1] = fadd2(sum[x & 1], e);
+            w[x] = pack_f16(e.x, e.y);
           }
-        }
-      }
-      const float2 f2 = make_float2(factor, factor), base2 = make_float2(kTop - m, kTop - m);
+        };
+        float2 both;
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+          sum[0] = sum[1] = make_float2(0.f, 0.f);
+          tmem_wait_ld_of(s0);
+          tmem_ld32(tm_s + 64 * half + 32, s1);
+          if (masked) mask(2 * half, s0);
+          weights(s0, p[0]);
+          tmem_wait_ld_of(s1);
+          if (masked) mask(2 * half + 1, s1);
+          weights(s1, p[1]);
+          both = fadd2(sum[0], sum[1]);
+          // a weight too large for fp16 makes the sum larger than 2^15 (and where it is, one of the 64 is 2^9 at least); so does a NaN
+          const bool bad = !(both.x + both.y <= 32768.f) || m == kLowest;
+          if (again || !__any_sync(0xffffffffu, bad)) break;
+          // once more with the maximum of these 64 scores.  Rows that are well get the same weights again: no row's bits depend on
+          // another row.
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i) {
+            tmem_ld32(tm_s + 64 * half + 32 * i, s1);
+            tmem_wait_ld_of(s1);
+            if (masked) mask(2 * half + i, s1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t p[16];
+            for (int x = 0; x < 32; x += 2) top = fmaxf(top, fmaxf(__uint_as_float(s1[x]), __uint_as_float(s1[x + 1])));
+          }
+          const float m_new = bad ? fmaxf(m, top * factor) : m, corr = ex2_approx(m - m_new);
+          m = m_new;
+          l.x *= corr; l.y *= corr;
+          if (j > 0 || half == 1) {
+            fail = half == 0 ? wait_bar<67>(bars + Bar::pv_done + 8 * t, (j - 1) & 1) : wait_bar<67>(bars + Bar::pv_half + 8 * t, j & 1);
+            if (fail != 0) return;
+            tc_fence_after();
+#pragma unroll 1
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld16(tm_o + 16 * i, o);
+              tmem_wait_ld();
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          float2 e = ffma2(make_float2(__uint_as_float(s[i][2 * x]), __uint_as_float(s[i][2 * x + 1])), f2, base2);
-          e.x = ex2_approx(e.x); e.y = ex2_approx(e.y);
-          l = fadd2(l, e);
-          p[x] = pack_f16(e.x, e.y);
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+              tmem_st16(tm_o + 16 * i, o);
+            }
+          }
+          tmem_ld32(tm_s + 64 * half, s0);
         }
-        tmem_st16(tm_s + 16 * i, p);
+        l = fadd2(l, both);
+        tmem_st16(tm_s + 32 * half, p[0]);
+        tmem_st16(tm_s + 32 * half + 16, p[1]);
+        if (half == 0) tmem_ld32(tm_s + 64, s0);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + Bar::p_full + 16 * half + 8 * t);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bars + Bar::p_full + 8 * t);
-    }
+    };
+    const int plain = absent ? 0 : max(0, min(count, (limit_all - key_begin) / kN));     // tiles all of whose keys every row of the warp sees
+    int j = 0;
+#pragma unroll 1
+    for (; j < plain && fail == 0; ++j) key_tile(Int<0>{}, j);
+#pragma unroll 1
+    for (; j < count && fail == 0; ++j) key_tile(Int<1>{}, j);
     if (fail == 0 && count > 0) fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (count - 1) & 1);
     if (fail != 0) {
       give_up(abort_s, P.status, fail);
@@ -525,7 +582,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
