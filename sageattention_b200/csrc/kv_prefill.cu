@@ -18,7 +18,8 @@
 //
 // Every wait on an mbarrier is bounded; where one gives up the CTA records its code in *status, waits (bounded) for its MMAs in
 // flight, frees its tensor memory and returns: 60 K stage free, 61 V stage free, 62 Q there, 63 K there, 64 V there, 65 P there, 66 scores
-// there, 67 last P V done; 68 tensor memory begins elsewhere.
+// there, 67 last P V done; 68 tensor memory begins elsewhere; 69 records
+// there.
 #include "kv_attn.cuh"
 
 namespace sage3 {
@@ -46,7 +47,7 @@ struct Lay {                              // shared memory
   static __device__ __forceinline__ int at(int row, int chunk) { return (chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 };
 struct Bar {                              // byte offsets in the barrier block, of two each but for p_full and the last
-  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96 /* [half][tile] */, pv_half = 128, pv_done = 144, drain = 160, tmem = 176, abort = 184;
+  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96 /* [half][tile] */, pv_half = 128, pv_done = 144, drain = 160, tmem = 168, abort = 176, raw = 184 /* [warp] */;
 };
 
 struct Params2 {
@@ -88,10 +89,6 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo
 __device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&x)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
 }
-__device__ __forceinline__ void lds(uint32_t at, uint32_t (&x)[4]) {
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
-}
-__device__ __forceinline__ void lds(uint32_t at, uint32_t (&x)[2]) { asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at)); }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -107,8 +104,6 @@ __device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
                :: "memory");
   asm volatile("" : "+r"(r[30]), "+r"(r[31]));
 }
-__device__ __forceinline__ uint32_t splat(uint32_t pair, bool hi) { return __byte_perm(pair, 0, hi ? 0x3232 : 0x1010); }
-
 // fp16 x fp16 -> fp32, A K-major, B K-major or (transposed) MN-major
 __host__ __device__ constexpr uint32_t idesc_f16(int N, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kM >> 4) << 24); }
 
@@ -170,8 +165,10 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       mbar_init(bars + Bar::p_full + 16 + 8 * i, 4);
       mbar_init(bars + Bar::pv_half + 8 * i, 1);
       mbar_init(bars + Bar::pv_done + 8 * i, 1);
-      mbar_init(bars + Bar::drain + 8 * i, 1);
     }
+    mbar_init(bars + Bar::drain, 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mbar_init(bars + Bar::raw + 8 * i, 1);
     *abort_s = 0;
     fence_mbar_init();
   }
@@ -196,19 +193,12 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       // (tensor memory begins at 0, all of it being this CTA's, and stages and tiles are unrolled: addresses are constants)
       auto scores = [&](auto t_, auto stage_) {
         constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value;
-        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
-            mma_f16_ss(t * kN, q_lo + t * (L::kOperand >> 4) + off, k_lo + stage * (L::kOperand >> 4) + off, HI, idesc_s, kk > 0);
-          }
-          tc_commit(bars + Bar::s_full + 8 * t);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
+          mma_f16_ss(t * kN, q_lo + t * (L::kOperand >> 4) + off, k_lo + stage * (L::kOperand >> 4) + off, HI, idesc_s, kk > 0);
         }
-        __syncwarp();
-      };
-      auto commit = [&](int bar) {
-        if (elect_one()) tc_commit(bars + bar);
-        __syncwarp();
+        tc_commit(bars + Bar::s_full + 8 * t);
       };
       const int count0 = R.count[0], count1 = R.count[1];
       if (tmem != 0) fail = 68;
@@ -218,42 +208,50 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
         fail = wait_bar<63>(bars + Bar::k_full, 0);
         if (fail == 0) {
           tc_fence_after();
-          if (count0 > 0) scores(Int<0>{}, Int<0>{});
-          if (count1 > 0) scores(Int<1>{}, Int<0>{});
-          commit(Bar::k_empty);
-        }
-      }
-      auto tile = [&](auto t_, auto stage_, int j, int count, bool& have_v, bool& have_k) {
-        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value, next = stage ^ 1;
-        if (fail != 0 || j >= count) return;
-        if (!have_v && (fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1)) != 0) return;
-        have_v = true;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if ((fail = wait_bar<65>(bars + Bar::p_full + 16 * half + 8 * t, j & 1)) != 0) return;
-          tc_fence_after();
           if (elect_one()) {
-#pragma unroll
-            for (int kk = half * (kN / 32); kk < (half + 1) * (kN / 32); ++kk)
-              mma_f16_ts(256 + t * 128, t * kN + kk * 8, v_lo + stage * (L::kOperand >> 4) + kk * (2048 >> 4), HI, idesc_o, kk > 0 ? 1u : j > 0);
-            tc_commit(bars + (half ? Bar::pv_done : Bar::pv_half) + 8 * t);
+            if (count0 > 0) scores(Int<0>{}, Int<0>{});
+            if (count1 > 0) scores(Int<1>{}, Int<0>{});
+            tc_commit(bars + Bar::k_empty);
           }
           __syncwarp();
         }
-        if (j + 1 >= count) return;
-        if (!have_k && (fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1)) != 0) return;
-        have_k = true;
+      }
+      auto values = [&](auto t_, auto stage_, auto half_, int j) {                        // 64 keys' part of P V
+        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value, half = decltype(half_)::value;
+#pragma unroll
+        for (int kk = half * (kN / 32); kk < (half + 1) * (kN / 32); ++kk)
+          mma_f16_ts(256 + t * 128, t * kN + kk * 8, v_lo + stage * (L::kOperand >> 4) + kk * (2048 >> 4), HI, idesc_o, kk > 0 ? 1u : j > 0);
+        tc_commit(bars + (half ? Bar::pv_done : Bar::pv_half) + 8 * t);
+      };
+      auto tile = [&](auto t_, auto stage_, int j, int count) {
+        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value, next = stage ^ 1;
+        if (fail != 0 || j >= count) return;
+        const bool more = j + 1 < count;
+        // (what has long been there is looked at first: behind the last part of P the next scores then follow at once)
+        if ((fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1)) != 0) return;
+        if (more && (fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1)) != 0) return;
+        if ((fail = wait_bar<65>(bars + Bar::p_full + 8 * t, j & 1)) != 0) return;
         tc_fence_after();
-        scores(t_, Int<next>{});
+        if (elect_one()) values(t_, stage_, Int<0>{}, j);
+        __syncwarp();
+        if ((fail = wait_bar<65>(bars + Bar::p_full + 16 + 8 * t, j & 1)) != 0) return;
+        tc_fence_after();
+        if (elect_one()) {
+          values(t_, stage_, Int<1>{}, j);
+          if (more) scores(t_, Int<next>{});
+        }
+        __syncwarp();
       };
       auto step = [&](auto stage_, int j) {
         constexpr int stage = decltype(stage_)::value;
-        bool have_v = false, have_k = false;
-        tile(Int<0>{}, stage_, j, count0, have_v, have_k);
-        tile(Int<1>{}, stage_, j, count1, have_v, have_k);
+        tile(Int<0>{}, stage_, j, count0);
+        tile(Int<1>{}, stage_, j, count1);
         if (fail != 0) return;
-        commit(Bar::v_empty + 8 * stage);
-        if (have_k) commit(Bar::k_empty + 8 * (stage ^ 1));
+        if (elect_one()) {
+          tc_commit(bars + Bar::v_empty + 8 * stage);
+          if (j + 1 < steps) tc_commit(bars + Bar::k_empty + 8 * (stage ^ 1));
+        }
+        __syncwarp();
       };
 #pragma unroll 1
       for (int j = 0; j < steps && fail == 0; j += 2) {
@@ -262,7 +260,8 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       }
       if (fail != 0) {
         give_up(abort_s, P.status, fail);
-        commit(Bar::drain);
+        if (elect_one()) tc_commit(bars + Bar::drain);
+        __syncwarp();
         mbar_wait<true>(bars + Bar::drain, 0, 1u << 16);
       }
     }
@@ -276,8 +275,8 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
     const bool halves = A.page_size < 32;
     int ids0 = -1, ids1 = -1;                                  // page ids of 32 tiles, one per lane
     const int part = keys ? L::kKeyPart : L::kValuePart;
-    const uint32_t raw_at = base + (keys ? L::raw_k : L::raw_v) + 2 * w * part;
-    // this warp's part of two records of tile j on its way to the raw buffer; zeros where there is no page or no key that is seen
+    const uint32_t raw_at = base + (keys ? L::raw_k : L::raw_v) + 2 * w * part, bar_raw = bars + Bar::raw + 8 * (warp - 8);
+    // this warp's part of two records of tile j on its way to the raw buffer, where there is a page and a key that is seen; says which
     auto fetch = [&](int j) {
       const int key = key_begin + j * kN + w * 32;
       if ((j & 31) == 0) {
@@ -287,41 +286,54 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       }
       const int p0 = __shfl_sync(0xffffffffu, ids0, j & 31), p1 = halves ? __shfl_sync(0xffffffffu, ids1, j & 31) : p0;
       const bool ok0 = (uint32_t)p0 < (uint64_t)A.num_pages, ok1 = (uint32_t)p1 < (uint64_t)A.num_pages && key + 16 < key_end;
-      const uint8_t* const r0 = head + (ok0 ? p0 * page_bytes + ((key & (A.page_size - 1)) >> 4) * Rec::kBytes : 0);
-      const uint8_t* const r1 = halves ? head + (ok1 ? p1 * page_bytes : 0) : r0 + (ok1 ? Rec::kBytes : 0);
-      constexpr int kMost = 2 * L::kKeyPart;
-#pragma unroll
-      for (int x = 0; x < kMost; x += 512) {
-        const int at = x + lane * 16;
-        if (at < 2 * part) {
-          const bool second = at >= part, ok = second ? ok1 : ok0;
-          const int in = second ? at - part : at;
-          const int off = keys ? (in < Rec::kValues ? in : in + (Rec::kValueScales - Rec::kValues)) : in + Rec::kValues;
-          cp_async16(raw_at + at, ok ? (second ? r1 : r0) + off : head, ok);
+      if (elect_one()) {
+        mbar_arrive_expect_tx(bar_raw, ((ok0 ? 1 : 0) + (ok1 ? 1 : 0)) * part);
+        const uint8_t* const r0 = head + (p0 * page_bytes + ((key & (A.page_size - 1)) >> 4) * Rec::kBytes);
+        const uint8_t* const r1 = halves ? head + p1 * page_bytes : r0 + Rec::kBytes;
+        if (ok0) {
+          bulk_load(raw_at, keys ? r0 : r0 + Rec::kValues, Rec::kValues, bar_raw);
+          if (keys) bulk_load(raw_at + Rec::kValues, r0 + Rec::kValueScales, D, bar_raw);
+        }
+        if (ok1) {
+          bulk_load(raw_at + part, keys ? r1 : r1 + Rec::kValues, Rec::kValues, bar_raw);
+          if (keys) bulk_load(raw_at + part + Rec::kValues, r1 + Rec::kValueScales, D, bar_raw);
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      __syncwarp();
+      return (ok0 ? 1 : 0) | (ok1 ? 2 : 0);
     };
     constexpr int W = D / 32;                                  // words of a lane's codes of a token (keys), of two tokens (values)
-    const uint32_t scales_at = D == 128 ? lane * 4 : (lane >> 3) * 16 + c * 4;
-    if (steps > 0) fetch(0);
+    // D=128: half of the lanes take the halves of their 16 bytes in the other order, so that 8 lanes' stores meet different banks.  Keys:
+    // rows n, n + 1 and channels 32 c ... fall on the same 128 bytes for c and c + 2.  Values: blocks n and n + 1 do.
+    const bool turn = D == 128 && (keys ? c >= 2 : n & 1);
+    const uint32_t codes_at = raw_at + lane * 4 * W, first = turn ? 8 : 0, second = turn ? 0 : 8;
+    const uint32_t scales_at = raw_at + (keys ? Rec::kValues : Rec::kValueScales - Rec::kValues) + (D == 128 ? lane * 4 : (lane >> 3) * 16 + c * 4);
+    int there = steps > 0 ? fetch(0) : 0;
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
       const int stage = j & 1, key0 = key_begin + j * kN + w * 32;
       // all of it to registers, and the next on its way
-      cp_async_wait_all();
-      __syncwarp();
+      if ((fail = wait_bar<69>(bar_raw, j & 1)) != 0) break;
       uint32_t x[2][2][W], ks[2] = {0, 0}, vsc[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t rec = raw_at + r * part;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) lds(rec + i * 4 * D + lane * 4 * W, x[r][i]);
-        vsc[r] = lds32(rec + (keys ? Rec::kValues : Rec::kValueScales - Rec::kValues) + scales_at);
-        if (keys) ks[r] = D == 128 ? lds32(rec + Rec::kKeyScales + lane * 4) : lds16(rec + Rec::kKeyScales + lane * 2);
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t at = codes_at + r * part + i * 4 * D;
+          if constexpr (D == 128) {
+            const uint2 u = lds64(at + first), v = lds64(at + second);
+            x[r][i][0] = u.x; x[r][i][1] = u.y; x[r][i][2] = v.x; x[r][i][3] = v.y;
+          } else {
+            const uint2 u = lds64(at);
+            x[r][i][0] = u.x; x[r][i][1] = u.y;
+          }
+        }
+        vsc[r] = lds32(scales_at + r * part);
+        if (keys) ks[r] = D == 128 ? lds32(raw_at + r * part + Rec::kKeyScales + lane * 4) : lds16(raw_at + r * part + Rec::kKeyScales + lane * 2);
+        if (!(there >> r & 1)) ks[r] = vsc[r] = 0;             // (zeros, then; a page there is not masks its keys as well)
       }
       __syncwarp();
-      if (j + 1 < steps) fetch(j + 1);
+      if (j + 1 < steps) there = fetch(j + 1);
       if (j >= 2) {
         fail = keys ? wait_bar<60>(bars + Bar::k_empty + 8 * stage, ((j >> 1) - 1) & 1) : wait_bar<61>(bars + Bar::v_empty + 8 * stage, ((j >> 1) - 1) & 1);
         if (fail != 0) break;
@@ -334,9 +346,6 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
           vsc[r] = u.x; poison = u.y;
         }
         if (keys) {
-          // Lanes 2 and 3 of a quad (D=128) take their words in another order, so that 8 lanes' stores meet different banks: those of
-          // rows n and n + 1 and channels 32 c ... fall on the same 128 bytes for c and c + 2.
-          const bool turn = D == 128 && c >= 2;
           const uint32_t sk = base + L::k + stage * L::kOperand;
           const uint32_t f0 = e4m3x2_to_f16(ks[r]), f1 = D == 128 ? e4m3x2_to_f16(ks[r] >> 16) : f0;
 #pragma unroll
@@ -344,34 +353,33 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
             const int row = w * 32 + r * 16 + i * 8 + n;
             uint32_t sc[2];
             if constexpr (D == 128) {
-              sc[0] = splat(i ? f1 : f0, turn); sc[1] = splat(i ? f1 : f0, !turn);
+              sc[0] = __byte_perm(i ? f1 : f0, 0, turn ? 0x3232 : 0x1010); sc[1] = __byte_perm(i ? f1 : f0, 0, turn ? 0x1010 : 0x3232);
             } else {
-              sc[0] = sc[1] = splat(f0, i);
+              sc[0] = sc[1] = __byte_perm(f0, 0, i ? 0x3232 : 0x1010);
             }
             if (poison >> i & 1) sc[0] = sc[1] = 0x7e007e00u;
 #pragma unroll
             for (int z = 0; z < W; ++z) {
               uint32_t y[4];
-              e2m1x8_to_f16(D == 128 && turn ? x[r][i][z ^ 2] : x[r][i][z], y);
+              e2m1x8_to_f16(x[r][i][z], y);
 #pragma unroll
               for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc[D == 128 ? z >> 1 : 0]);
-              sts128(sk + L::at(row, c * W + (D == 128 && turn ? z ^ 2 : z)), y);
+              sts128(sk + L::at(row, c * W + (turn ? z ^ 2 : z)), y);
             }
           }
         } else {
           const uint32_t sv = base + L::v + stage * L::kOperand;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {                        // tokens 2 c + 8 i and the next; odd n (D=128) the other way round
+          for (int i = 0; i < 2; ++i) {                        // tokens 2 c + 8 i and the next, or (turn) the other way round
             const uint32_t f = e4m3x2_to_f16(vsc[r] >> (16 * i));
-            const bool turn = D == 128 && (n & 1);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int row = w * 32 + r * 16 + i * 8 + 2 * c + (turn ? e ^ 1 : e);
-              const uint32_t sc = splat(f, turn ? e == 0 : e == 1);
+              const uint32_t sc = __byte_perm(f, 0, (turn ? e == 0 : e == 1) ? 0x3232 : 0x1010);
 #pragma unroll
               for (int z = 0; z < W / 2; ++z) {
                 uint32_t y[4];
-                e2m1x8_to_f16(turn ? x[r][i][(e ^ 1) * (W / 2) + z] : x[r][i][e * (W / 2) + z], y);
+                e2m1x8_to_f16(x[r][i][e * (W / 2) + z], y);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc);
                 sts128(sv + L::at(row, n * (W / 2) + z), y);
@@ -384,8 +392,10 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + (keys ? Bar::k_full : Bar::v_full) + 8 * stage);
     }
-    cp_async_wait_all();
-    if (fail != 0) give_up(abort_s, P.status, fail);
+    if (fail != 0) {
+      give_up(abort_s, P.status, fail);
+      for (int x = 0; x < 2; ++x) mbar_wait<true>(bar_raw, x, 1u << 16);     // its copy in flight, if any: one of the two phases is past
+    }
   } else {
     // ---------------------------------------------------------------- softmax: thread r of the warpgroup has row r of its tile
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -489,7 +499,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
           both = fadd2(sum[0], sum[1]);
           // a weight too large for fp16 makes the sum larger than 2^15 (and where it is, one of the 64 is 2^9 at least); so does a NaN
           const bool bad = !(both.x + both.y <= 32768.f) || m == kLowest;
-          if (again || !__any_sync(0xffffffffu, bad)) break;
+          if (__builtin_expect(again || !__any_sync(0xffffffffu, bad), 1)) break;
           // once more with the maximum of these 64 scores.  Rows that are well get the same weights again: no row's bits depend on
           // another row.
           float top = -INFINITY;
