@@ -205,7 +205,7 @@ struct KvAttnArgs {
 size_t kv_decode_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms);
 bool kv_decode_fits(int B, int Hq, int Hkv, int max_q, int max_k);  // its counts stay within 32 bits
 cudaError_t launch_kv_decode(const KvAttnArgs& a, cudaStream_t stream);
-bool kv_prefill_takes(int Hq, int Hkv, int DS, int max_q, int max_k);      // the faster of the two
+bool kv_prefill_takes(int Hq, int Hkv, int DS, int max_q);         // the faster of the two
 size_t kv_prefill_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms);
 bool kv_prefill_fits(int B, int Hq, int Hkv, int max_q);
 cudaError_t launch_kv_prefill(const KvAttnArgs& a, cudaStream_t stream);

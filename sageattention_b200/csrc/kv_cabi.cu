@@ -30,7 +30,7 @@ sage3::KvRows rows_of(const sage3_tensor& t) { return sage3::KvRows{t.ptr, t.str
 inline int longest_q(const sage3_kv_attention_args* a) { return a->cu_seqlens_q != nullptr ? a->max_seqlen_q : 1; }
 
 inline bool takes_prefill(const sage3_kv_attention_args* a) {
-  return sage3::kv_prefill_takes(a->Hq, a->cache->num_kv_heads, a->cache->head_dim_stored, longest_q(a), a->max_seqlen_k);
+  return sage3::kv_prefill_takes(a->Hq, a->cache->num_kv_heads, a->cache->head_dim_stored, longest_q(a));
 }
 
 int check_attention(const sage3_kv_attention_args* a) {

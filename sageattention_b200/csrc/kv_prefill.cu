@@ -1,10 +1,11 @@
 // Attention of many query rows per kv head over the 4-bit cache: chunks of prompts behind cached prefixes.
 //
 // A CTA takes 256 rows (tokens times the heads of a kv head, two tiles of 128) of a (sequence, kv head) and walks tiles of 128 keys:
-//   warps 8-11   fetch the keys' part of the records as it is, turn codes and scales into fp16 (exact, see kv_decode.cu) and write K
+//   warps 8-11   read the keys' part of the records, turn codes and scales into fp16 (exact, see kv_decode.cu) and write K
 //                tiles to shared memory, once for all 256 rows
 //   warps 12-15  the same with values.  Both tiles lie alike, rows of keys with 128-byte swizzle: K is then the K-major B operand of
 //                S = Q K^T and V the MN-major one of O += P V, so nothing is transposed
+//   warp  17     fetches the records by bulk copies
 //   warp  16     issues the tcgen05.mma kind::f16: S_t = Q_t K^T (queries from shared memory), O_t += P_t V (P from tensor memory)
 //   warps 0-3    softmax of row tile 0, a thread per row: scores from tensor memory to registers, weights back over them in fp16
 //   warps 4-7    the same for row tile 1; one tile's softmax runs beside the other's MMAs
@@ -19,7 +20,7 @@
 // Every wait on an mbarrier is bounded; where one gives up the CTA records its code in *status, waits (bounded) for its MMAs in
 // flight, frees its tensor memory and returns: 60 K stage free, 61 V stage free, 62 Q there, 63 K there, 64 V there, 65 P there, 66 scores
 // there, 67 last P V done; 68 tensor memory begins elsewhere; 69 records
-// there.
+// there, 71 records read.
 #include "kv_attn.cuh"
 
 namespace sage3 {
@@ -40,14 +41,13 @@ template <int D>
 struct Lay {                              // shared memory
   static constexpr int kOperand = kM * D * 2, kHalf = kM * 128;      // a tile; its part of 64 channels
   static constexpr int q = 0, k = 2 * kOperand, v = 4 * kOperand;
-  // parts of a tile's records as they are, two per warp: keys with both kinds of scales, and values with theirs
-  static constexpr int kKeyPart = 10 * D, kValuePart = 9 * D, raw_k = 6 * kOperand, raw_v = raw_k + 8 * kKeyPart, kRaw = 8 * (kKeyPart + kValuePart), raw = raw_k;
+  static constexpr int raw = 6 * kOperand, kRaw = kN / 16 * 18 * D;  // a tile's records as they are
   static constexpr int bars = raw + kRaw, total = bars + 256;
   // 16 bytes: channels 8 chunk ... of a row
   static __device__ __forceinline__ int at(int row, int chunk) { return (chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 };
 struct Bar {                              // byte offsets in the barrier block, of two each but for p_full and the last
-  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96 /* [half][tile] */, pv_half = 128, pv_done = 144, drain = 160, tmem = 168, abort = 176, raw = 184 /* [warp] */;
+  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96 /* [half][tile] */, pv_half = 128, pv_done = 144, drain = 160, raw_full = 168, raw_empty = 176, tmem = 184, abort = 192, there = 196;
 };
 
 struct Params2 {
@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       mbar_init(bars + Bar::pv_done + 8 * i, 1);
     }
     mbar_init(bars + Bar::drain, 1);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mbar_init(bars + Bar::raw + 8 * i, 1);
+    mbar_init(bars + Bar::raw_full, 1);
+    mbar_init(bars + Bar::raw_empty, 8);
     *abort_s = 0;
     fence_mbar_init();
   }
@@ -223,33 +223,40 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
           mma_f16_ts(256 + t * 128, t * kN + kk * 8, v_lo + stage * (L::kOperand >> 4) + kk * (2048 >> 4), HI, idesc_o, kk > 0 ? 1u : j > 0);
         tc_commit(bars + (half ? Bar::pv_done : Bar::pv_half) + 8 * t);
       };
+      // Looks at barriers are slow beside busy warps (150 cycles and more), and this warp is held up by the MMAs that it issues, so what a
+      // step needs of keys and values is looked at while the step before waits for weights; only if it is not there yet, again later.
+      bool have_v = false, have_k = false;                     // of the next step
+      auto look = [&](int j) {
+        if (j < steps && !have_v) have_v = __all_sync(0xffffffffu, mbar_test(bars + Bar::v_full + 8 * (j & 1), (j >> 1) & 1));
+        if (j + 1 < steps && !have_k) have_k = __all_sync(0xffffffffu, mbar_test(bars + Bar::k_full + 8 * ((j + 1) & 1), ((j + 1) >> 1) & 1));
+      };
       auto tile = [&](auto t_, auto stage_, int j, int count) {
         constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value, next = stage ^ 1;
         if (fail != 0 || j >= count) return;
-        const bool more = j + 1 < count;
-        // (what has long been there is looked at first: behind the last part of P the next scores then follow at once)
-        if ((fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1)) != 0) return;
-        if (more && (fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1)) != 0) return;
         if ((fail = wait_bar<65>(bars + Bar::p_full + 8 * t, j & 1)) != 0) return;
         tc_fence_after();
         if (elect_one()) values(t_, stage_, Int<0>{}, j);
         __syncwarp();
+        if (t == 1 || count1 == 0) look(j + 1);
         if ((fail = wait_bar<65>(bars + Bar::p_full + 16 + 8 * t, j & 1)) != 0) return;
         tc_fence_after();
         if (elect_one()) {
           values(t_, stage_, Int<1>{}, j);
-          if (more) scores(t_, Int<next>{});
+          if (j + 1 < count) scores(t_, Int<next>{});
         }
         __syncwarp();
       };
       auto step = [&](auto stage_, int j) {
-        constexpr int stage = decltype(stage_)::value;
+        constexpr int stage = decltype(stage_)::value, next = stage ^ 1;
+        if (!have_v) fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1);
+        if (fail == 0 && !have_k && j + 1 < steps) fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1);
+        have_v = have_k = false;
         tile(Int<0>{}, stage_, j, count0);
         tile(Int<1>{}, stage_, j, count1);
         if (fail != 0) return;
         if (elect_one()) {
           tc_commit(bars + Bar::v_empty + 8 * stage);
-          if (j + 1 < steps) tc_commit(bars + Bar::k_empty + 8 * (stage ^ 1));
+          if (j + 1 < steps) tc_commit(bars + Bar::k_empty + 8 * next);
         }
         __syncwarp();
       };
@@ -265,61 +272,63 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
         mbar_wait<true>(bars + Bar::drain, 0, 1u << 16);
       }
     }
+    else if (warp == 17) {
+      // ---------------------------------------------------------------- records, by bulk copies; which there are goes along
+      volatile uint32_t* const there_s = reinterpret_cast<volatile uint32_t*>(smem + L::bars + Bar::there);
+      const int64_t page_bytes = (int64_t)A.Hkv * (A.page_size / 16) * Rec::kBytes;
+      const uint8_t* const head = A.data + (int64_t)h * (A.page_size / 16) * Rec::kBytes;
+      auto page_of = [&](int j) {          // of record `lane` of tile j; -1: no page, or no key that is seen
+        const int key = key_begin + j * kN + 16 * lane;
+        if (lane >= kN / 16 || key >= key_end) return -1;
+        const int page = __ldg(table + (key >> P.page_shift));
+        return (uint32_t)page < (uint64_t)A.num_pages ? page : -1;
+      };
+      int page = steps > 0 ? page_of(0) : -1;
+#pragma unroll 1
+      for (int j = 0; j < steps; ++j) {
+        if (j > 0 && (fail = wait_bar<71>(bars + Bar::raw_empty, (j - 1) & 1)) != 0) break;
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) {
+          *there_s = there;
+          mbar_arrive_expect_tx(bars + Bar::raw_full, __popc(there) * Rec::kBytes);
+        }
+        __syncwarp();
+        const int key = key_begin + j * kN + 16 * lane;
+        if (page >= 0)
+          bulk_load(base + L::raw + lane * Rec::kBytes, head + page * page_bytes + ((key & (A.page_size - 1)) >> 4) * Rec::kBytes, Rec::kBytes, bars + Bar::raw_full);
+        __syncwarp();
+        page = j + 1 < steps ? page_of(j + 1) : -1;
+      }
+      if (fail != 0) {
+        give_up(abort_s, P.status, fail);
+        for (int x = 0; x < 2; ++x) mbar_wait<true>(bars + Bar::raw_full, x, 1u << 16);     // its copies in flight: one of the two phases is past
+      }
+    }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- cache -> fp16 tiles: a warp 32 keys of each
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFillRegs));
     const bool keys = warp < 12;
     const int w = warp & 3, n = lane >> 2, c = lane & 3;
-    const int64_t page_bytes = (int64_t)A.Hkv * (A.page_size / 16) * Rec::kBytes;
-    const uint8_t* const head = A.data + (int64_t)h * (A.page_size / 16) * Rec::kBytes;
-    const bool halves = A.page_size < 32;
-    int ids0 = -1, ids1 = -1;                                  // page ids of 32 tiles, one per lane
-    const int part = keys ? L::kKeyPart : L::kValuePart;
-    const uint32_t raw_at = base + (keys ? L::raw_k : L::raw_v) + 2 * w * part, bar_raw = bars + Bar::raw + 8 * (warp - 8);
-    // this warp's part of two records of tile j on its way to the raw buffer, where there is a page and a key that is seen; says which
-    auto fetch = [&](int j) {
-      const int key = key_begin + j * kN + w * 32;
-      if ((j & 31) == 0) {
-        const int mine = key + lane * kN;
-        ids0 = mine < key_end ? __ldg(table + (mine >> P.page_shift)) : -1;
-        if (halves) ids1 = mine + 16 < key_end ? __ldg(table + ((mine + 16) >> P.page_shift)) : -1;
-      }
-      const int p0 = __shfl_sync(0xffffffffu, ids0, j & 31), p1 = halves ? __shfl_sync(0xffffffffu, ids1, j & 31) : p0;
-      const bool ok0 = (uint32_t)p0 < (uint64_t)A.num_pages, ok1 = (uint32_t)p1 < (uint64_t)A.num_pages && key + 16 < key_end;
-      if (elect_one()) {
-        mbar_arrive_expect_tx(bar_raw, ((ok0 ? 1 : 0) + (ok1 ? 1 : 0)) * part);
-        const uint8_t* const r0 = head + (p0 * page_bytes + ((key & (A.page_size - 1)) >> 4) * Rec::kBytes);
-        const uint8_t* const r1 = halves ? head + p1 * page_bytes : r0 + Rec::kBytes;
-        if (ok0) {
-          bulk_load(raw_at, keys ? r0 : r0 + Rec::kValues, Rec::kValues, bar_raw);
-          if (keys) bulk_load(raw_at + Rec::kValues, r0 + Rec::kValueScales, D, bar_raw);
-        }
-        if (ok1) {
-          bulk_load(raw_at + part, keys ? r1 : r1 + Rec::kValues, Rec::kValues, bar_raw);
-          if (keys) bulk_load(raw_at + part + Rec::kValues, r1 + Rec::kValueScales, D, bar_raw);
-        }
-      }
-      __syncwarp();
-      return (ok0 ? 1 : 0) | (ok1 ? 2 : 0);
-    };
+    const uint32_t raw_at = base + L::raw + 2 * w * Rec::kBytes, codes_from = raw_at + (keys ? 0 : Rec::kValues);
+    const volatile uint32_t* const there_s = reinterpret_cast<const volatile uint32_t*>(smem + L::bars + Bar::there);
     constexpr int W = D / 32;                                  // words of a lane's codes of a token (keys), of two tokens (values)
     // D=128: half of the lanes take the halves of their 16 bytes in the other order, so that 8 lanes' stores meet different banks.  Keys:
     // rows n, n + 1 and channels 32 c ... fall on the same 128 bytes for c and c + 2.  Values: blocks n and n + 1 do.
     const bool turn = D == 128 && (keys ? c >= 2 : n & 1);
-    const uint32_t codes_at = raw_at + lane * 4 * W, first = turn ? 8 : 0, second = turn ? 0 : 8;
-    const uint32_t scales_at = raw_at + (keys ? Rec::kValues : Rec::kValueScales - Rec::kValues) + (D == 128 ? lane * 4 : (lane >> 3) * 16 + c * 4);
-    int there = steps > 0 ? fetch(0) : 0;
+    const uint32_t codes_at = codes_from + lane * 4 * W, first = turn ? 8 : 0, second = turn ? 0 : 8;
+    const uint32_t scales_at = raw_at + Rec::kValueScales + (D == 128 ? lane * 4 : (lane >> 3) * 16 + c * 4);
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
       const int stage = j & 1, key0 = key_begin + j * kN + w * 32;
-      // all of it to registers, and the next on its way
-      if ((fail = wait_bar<69>(bar_raw, j & 1)) != 0) break;
+      // two records to registers, so that the next can come
+      if ((fail = wait_bar<69>(bars + Bar::raw_full, j & 1)) != 0) break;
+      const uint32_t there = *there_s >> (2 * w);
       uint32_t x[2][2][W], ks[2] = {0, 0}, vsc[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t at = codes_at + r * part + i * 4 * D;
+          const uint32_t at = codes_at + r * Rec::kBytes + i * 4 * D;
           if constexpr (D == 128) {
             const uint2 u = lds64(at + first), v = lds64(at + second);
             x[r][i][0] = u.x; x[r][i][1] = u.y; x[r][i][2] = v.x; x[r][i][3] = v.y;
@@ -328,12 +337,12 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
             x[r][i][0] = u.x; x[r][i][1] = u.y;
           }
         }
-        vsc[r] = lds32(scales_at + r * part);
-        if (keys) ks[r] = D == 128 ? lds32(raw_at + r * part + Rec::kKeyScales + lane * 4) : lds16(raw_at + r * part + Rec::kKeyScales + lane * 2);
+        vsc[r] = lds32(scales_at + r * Rec::kBytes);
+        if (keys) ks[r] = D == 128 ? lds32(raw_at + r * Rec::kBytes + Rec::kKeyScales + lane * 4) : lds16(raw_at + r * Rec::kBytes + Rec::kKeyScales + lane * 2);
         if (!(there >> r & 1)) ks[r] = vsc[r] = 0;             // (zeros, then; a page there is not masks its keys as well)
       }
       __syncwarp();
-      if (j + 1 < steps) there = fetch(j + 1);
+      if (lane == 0) mbar_arrive(bars + Bar::raw_empty);
       if (j >= 2) {
         fail = keys ? wait_bar<60>(bars + Bar::k_empty + 8 * stage, ((j >> 1) - 1) & 1) : wait_bar<61>(bars + Bar::v_empty + 8 * stage, ((j >> 1) - 1) & 1);
         if (fail != 0) break;
@@ -392,10 +401,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + (keys ? Bar::k_full : Bar::v_full) + 8 * stage);
     }
-    if (fail != 0) {
-      give_up(abort_s, P.status, fail);
-      for (int x = 0; x < 2; ++x) mbar_wait<true>(bar_raw, x, 1u << 16);     // its copy in flight, if any: one of the two phases is past
-    }
+    if (fail != 0) give_up(abort_s, P.status, fail);
   } else {
     // ---------------------------------------------------------------- softmax: thread r of the warpgroup has row r of its tile
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -686,7 +692,10 @@ cudaError_t launch(const Params2& P, const Plan2& p, cudaStream_t stream) {
 
 }  // namespace
 
-bool kv_prefill_takes(int Hq, int Hkv, int DS, int max_q, int max_k) { return (int64_t)max_q * (Hq / Hkv) > 64; }
+// Rows per kv head from which on this kernel takes over.  kv_decode.cu turns a key's codes into fp16 once for 16 rows, this one once
+// for 256, but works on 128 rows at least.  Decode / prefill, B16 Hkv8 4096 keys: D=128 20 rows 54 / 58 us, 32 rows 57 / 58, 64 rows 93 / 59;
+// D=64 32 rows 36 / 49, 64 rows 57 / 49; B1 32768 keys, D=128: 20 rows 40 / 36, 64 rows 58 / 40.
+bool kv_prefill_takes(int Hq, int Hkv, int DS, int max_q) { return (int64_t)max_q * (Hq / Hkv) > (DS == 128 ? 32 : 48); }
 
 size_t kv_prefill_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) { return plan2(B, Hq, Hkv, DS, max_q, max_k, sms).bytes; }
 
