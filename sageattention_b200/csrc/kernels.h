@@ -173,8 +173,9 @@ struct KvTokensArgs {                     // norm, rotation, cache (kv_tokens.cu
   const void* k_offset;
   int page_size;
   int64_t num_slots;
+  int span;                               // heads per warp: set by the launch
 };
-cudaError_t launch_kv_tokens(const KvTokensArgs& a, cudaStream_t stream);
+cudaError_t launch_kv_tokens(KvTokensArgs a, cudaStream_t stream);
 
 struct KvReadArgs {
   const uint8_t* data;

@@ -106,195 +106,210 @@ cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Norm, rotation, cache.  One pass: a lane has 8 channels (16 bytes) of a row, 8 or 16 lanes a row (stored head dim 64 or 128), a warp
-// kRows rows of one token's heads at a time, all loaded before the first is used.  y = x rsqrt(mean(x^2) + eps) w in fp32; channel d < R
-// is turned with its partner (d + R/2, whose lane is asked for it, or the neighbour d ^ 1) by the token's angle; one rounding to bf16.
-// To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
+// Norm, rotation, cache.  One pass: a lane has 8 channels (16 bytes) of a row, 8 or 16 lanes a row (stored head dim 64 or 128).  A warp
+// takes a token's heads `span` at a time, kRows of them loaded before the first is used.
+//   y = x rsqrt(mean(x^2) + eps) w,   out = y cos - y' sin  or  y cos + y' sin,   y' the partner's (i +- R/2, or the neighbour i ^ 1)
+// What depends on the channel and the token alone, w cos and the partner's w sin, is worked out once for all heads, so a channel costs a
+// product, a fused one and the row's factor (975 -> 300 instructions for 8 rows of 128; N32760 H40/40 412 -> 226 us).  All in fp32, one rounding
+// to bf16.  To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
 // e4m3(max|x| / 6) over the two lanes of a block, code = e2m1(x / scale).  Bound by DRAM.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTokenThreads = 256;
 
 // 16-channel blocks to codes and scale; a lane has half a block.  x / scale is worked out as x * (1 / scale), rounded to fp16: x has 8
 // significant bits and a border between codes times the scale 7, so a quotient that is no border is 2^-8 from it, and one that is
-// comes out as the border itself (in fp32 alone some would miss it by a last bit, 5.25 / 7 for one, and round to the other side).
+// comes out as the border itself (in fp32 alone some would miss it by a last bit, 18.75 / 15 for one, and round to the other side).
 __device__ __forceinline__ void quant_half_block(const uint32_t (&x)[4], uint32_t& codes, uint32_t& scale) {
   uint32_t m2 = abs2(habsmax2(habsmax2(x[0], x[1]), habsmax2(x[2], x[3])));
   m2 = abs2(habsmax2(m2, __shfl_xor_sync(0xffffffffu, m2, 1)));
-  scale = f32_to_e4m3(__fdiv_rn(fmaxf(bf16_lo(m2), bf16_hi(m2)), 6.0f));
-  const float sf = e4m3_to_f32(scale), inv = sf == 0.f ? 0.f : __frcp_rn(sf);
+  float inv;
+  block_scale(fmaxf(bf16_lo(m2), bf16_hi(m2)), scale, inv);     // (its approximate operations are exact on bf16: tests/golden/device_tables)
+  const float2 inv2 = make_float2(inv, inv);
   float2 f[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = f16x2_to_f32(pack_f16(bf16_lo(x[i]) * inv, bf16_hi(x[i]) * inv));
+  for (int i = 0; i < 4; ++i) {
+    const float2 y = mul2_ftz(bf16x2_to_f32(x[i]), inv2);
+    f[i] = f16x2_to_f32(pack_f16(y.x, y.y));
+  }
   codes = f32x8_to_e2m1x8(f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y);
 }
 
 template <int DS>                         // stored head dim: 64 or 128
-__global__ void __launch_bounds__(kTokenThreads) kv_tokens_kernel(const KvTokensArgs A) {
+__global__ void __launch_bounds__(kTokenThreads, 4) kv_tokens_kernel(const KvTokensArgs A) {
   using Rec = KvRecord<DS>;
   constexpr int kLanes = DS / 8, kPerPass = 32 / kLanes, kPasses = 4, kRows = kPerPass * kPasses;
   const int lane = threadIdx.x & 31, l = lane % kLanes, sub = lane / kLanes;
-  const int gq = (A.Hq + kRows - 1) / kRows, gk = (A.Hkv + kRows - 1) / kRows;
-  const int groups = gq + gk + (A.v != nullptr ? gk : 0);
-  const int64_t item = (int64_t)blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5);
-  const int64_t token = item / groups;
-  if (token >= (int64_t)A.B * A.N) return;
-  int g = (int)(item - token * groups);
-  const int what = g < gq ? 0 : g < gq + gk ? 1 : 2;            // q, k, v
-  g -= what == 0 ? 0 : what == 1 ? gq : gq + gk;
-  const int b = (int)(token / A.N), n = (int)(token - (int64_t)b * A.N), heads = what == 0 ? A.Hq : A.Hkv;
+  const int token = blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5);
+  if (token >= A.B * A.N) return;
+  const int gq = (A.Hq + A.span - 1) / A.span, gk = (A.Hkv + A.span - 1) / A.span;
+  const int g = blockIdx.y, what = g < gq ? 0 : g < gq + gk ? 1 : 2;                 // q, k, v
+  const int heads = what == 0 ? A.Hq : A.Hkv, h0 = (what == 0 ? g : what == 1 ? g - gq : g - gq - gk) * A.span, h1 = min(h0 + A.span, heads);
+  const int b = A.B == 1 ? 0 : token / A.N, n = token - b * A.N;
   const KvRows& in = what == 0 ? A.q : what == 1 ? A.k : A.vr;
-  const __nv_bfloat16* const src = (const __nv_bfloat16*)in.ptr + b * in.sb + n * in.sn;
   const bool have = l * 8 < A.D;                                // stored channels beyond the head dim are zero
-
-  uint4 x[kPasses];
-#pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int h = g * kRows + p * kPerPass + sub;
-    x[p] = make_uint4(0, 0, 0, 0);
-    if (have && h < heads) x[p] = __ldg(reinterpret_cast<const uint4*>(src + h * in.sh + l * 8));
-  }
+  const __nv_bfloat16* const src = (const __nv_bfloat16*)in.ptr + b * in.sb + n * in.sn + l * 8;
+  const bool to_cache = what != 0 && A.data != nullptr;
   int64_t slot = -1;
-  if (what != 0 && A.data != nullptr) {
+  if (to_cache) {
     slot = __ldg(A.slots + token);
     if (slot < 0 || slot >= A.num_slots) slot = -1;
   }
 
-  if (what != 2 && (A.weight[what] != nullptr || A.rot > 0)) {
-    const __nv_bfloat16* const weight = (const __nv_bfloat16*)A.weight[what];
-    const int quads = A.rot / 8;                                // groups of 4 channels in half of the rotated ones
-    const bool turned = l * 8 < A.rot;
-    // channels in pairs of words; the partner of group 2 l + s of 4 channels is group (2 l + s +- quads), in lane src_lane[s]
-    float w[8], cs[8], sn[8], pw[8];
-    int src_lane[2] = {lane, lane}, odd = 0;
+  // ---- what the channels of this token are multiplied by: themselves (own), and their partners (other)
+  const bool normed = what != 2 && A.weight[what] != nullptr, turned = what != 2 && l * 8 < A.rot, change = what != 2 && (normed || A.rot > 0);
+  const int quads = A.rot / 8;                                  // groups of 4 channels in half of the rotated ones
+  const bool halves = what != 2 && A.rot > 0 && !A.adjacent;
+  float own[8], other[8];
+  int src_lane[2] = {lane, lane};                               // of the partners of group 2 l + s of 4 channels (halves)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { w[i] = pw[i] = 1.f; cs[i] = 1.f; sn[i] = 0.f; }
-    if (weight != nullptr && have) {
+  for (int i = 0; i < 8; ++i) { own[i] = 1.f; other[i] = 0.f; }
+  if (change) {
+    const __nv_bfloat16* const weight = (const __nv_bfloat16*)A.weight[what];
+    float w[8], pw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pw[i] = 1.f;
+    if (normed && have) {
       const uint4 u = __ldg(reinterpret_cast<const uint4*>(weight + l * 8));
       w[0] = bf16_lo(u.x); w[1] = bf16_hi(u.x); w[2] = bf16_lo(u.y); w[3] = bf16_hi(u.y);
       w[4] = bf16_lo(u.z); w[5] = bf16_hi(u.z); w[6] = bf16_lo(u.w); w[7] = bf16_hi(u.w);
     }
-    if (A.rot > 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) own[i] = w[i];
+    if (turned) {
       int64_t place = n;
       if (A.positions != nullptr) place = A.positions64 ? __ldg((const int64_t*)A.positions + token) : (int64_t)__ldg((const int*)A.positions + token);
       const bool known = place >= 0 && place < A.places;        // outside the table: NaN, so that it shows
-      odd = quads & 1;
-      if (turned) {
-        const int half = A.rot / 2;
+      const int half = A.rot / 2;
+      const float *const cos = A.cos + place * half, *const sin = A.sin + place * half;
+      if (A.adjacent) {                                         // pairs (8 l + 2 i, + 1): one angle for two channels
+        float4 c4 = make_float4(NAN, NAN, NAN, NAN), s4 = c4;
+        if (known) {
+          c4 = __ldg(reinterpret_cast<const float4*>(cos + l * 4));
+          s4 = __ldg(reinterpret_cast<const float4*>(sin + l * 4));
+        }
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          own[2 * i] = w[2 * i] * c[i]; own[2 * i + 1] = w[2 * i + 1] * c[i];
+          other[2 * i] = -w[2 * i + 1] * s[i]; other[2 * i + 1] = w[2 * i] * s[i];
+        }
+      } else {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const int u = 2 * l + s;
+          const int u = 2 * l + s, pu = u >= quads ? u - quads : u + quads, angle = u >= quads ? pu : u;
           float4 c4 = make_float4(NAN, NAN, NAN, NAN), s4 = c4;
-          if (A.adjacent) {
-            // pairs (8 l + 2 i, + 1): one angle for two channels
-            if (known && s == 0) {
-              c4 = __ldg(reinterpret_cast<const float4*>(A.cos + place * half + l * 4));
-              s4 = __ldg(reinterpret_cast<const float4*>(A.sin + place * half + l * 4));
-            }
-            if (s == 0) {
-              cs[0] = cs[1] = c4.x; cs[2] = cs[3] = c4.y; cs[4] = cs[5] = c4.z; cs[6] = cs[7] = c4.w;
-              sn[0] = -s4.x; sn[1] = s4.x; sn[2] = -s4.y; sn[3] = s4.y; sn[4] = -s4.z; sn[5] = s4.z; sn[6] = -s4.w; sn[7] = s4.w;
-            }
-          } else {
-            const bool upper = u >= quads;
-            const int pu = upper ? u - quads : u + quads;
-            if (known) {
-              c4 = __ldg(reinterpret_cast<const float4*>(A.cos + place * half + (upper ? pu : u) * 4));
-              s4 = __ldg(reinterpret_cast<const float4*>(A.sin + place * half + (upper ? pu : u) * 4));
-            }
-            const float sign = upper ? 1.f : -1.f;
-            cs[4 * s] = c4.x; cs[4 * s + 1] = c4.y; cs[4 * s + 2] = c4.z; cs[4 * s + 3] = c4.w;
-            sn[4 * s] = sign * s4.x; sn[4 * s + 1] = sign * s4.y; sn[4 * s + 2] = sign * s4.z; sn[4 * s + 3] = sign * s4.w;
-            src_lane[s] = lane - l + (pu >> 1);
-            if (weight != nullptr) {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(weight + pu * 4));
-              pw[4 * s] = bf16_lo(v.x); pw[4 * s + 1] = bf16_hi(v.x); pw[4 * s + 2] = bf16_lo(v.y); pw[4 * s + 3] = bf16_hi(v.y);
-            }
+          if (known) {
+            c4 = __ldg(reinterpret_cast<const float4*>(cos + angle * 4));
+            s4 = __ldg(reinterpret_cast<const float4*>(sin + angle * 4));
+          }
+          src_lane[s] = lane - l + (pu >> 1);
+          if (normed) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(weight + pu * 4));
+            pw[4 * s] = bf16_lo(v.x); pw[4 * s + 1] = bf16_hi(v.x); pw[4 * s + 2] = bf16_lo(v.y); pw[4 * s + 3] = bf16_hi(v.y);
+          }
+          const float c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w}, sign = u >= quads ? 1.f : -1.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            own[4 * s + i] = w[4 * s + i] * c[i];
+            other[4 * s + i] = sign * pw[4 * s + i] * sn[i];
           }
         }
       }
-    }
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      float f[8] = {bf16_lo(x[p].x), bf16_hi(x[p].x), bf16_lo(x[p].y), bf16_hi(x[p].y),
-                    bf16_lo(x[p].z), bf16_hi(x[p].z), bf16_lo(x[p].w), bf16_hi(x[p].w)};
-      float r = 1.f;
-      if (weight != nullptr) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(f[i], f[i], s);
-#pragma unroll
-        for (int d = 1; d < kLanes; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-        r = 1.0f / sqrtf(s * A.inv_d + A.eps);
-      }
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = f[i] * r * w[i];
-      if (A.rot > 0) {
-        float o[8];
-        if (A.adjacent) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = y[i ^ 1];
-        } else {
-          // the partner's raw words; with an odd number of quads its other half is meant
-          uint32_t a0 = __shfl_sync(0xffffffffu, x[p].x, src_lane[0]), a1 = __shfl_sync(0xffffffffu, x[p].y, src_lane[0]);
-          uint32_t b0 = __shfl_sync(0xffffffffu, x[p].z, src_lane[1]), b1 = __shfl_sync(0xffffffffu, x[p].w, src_lane[1]);
-          if (odd) {
-            a0 = __shfl_sync(0xffffffffu, x[p].z, src_lane[0]); a1 = __shfl_sync(0xffffffffu, x[p].w, src_lane[0]);
-            b0 = __shfl_sync(0xffffffffu, x[p].x, src_lane[1]); b1 = __shfl_sync(0xffffffffu, x[p].y, src_lane[1]);
-          }
-          const float raw[8] = {bf16_lo(a0), bf16_hi(a0), bf16_lo(a1), bf16_hi(a1), bf16_lo(b0), bf16_hi(b0), bf16_lo(b1), bf16_hi(b1)};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = raw[i] * r * pw[i];
-        }
-        if (turned)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = y[i] * cs[i] + o[i] * sn[i];
-      }
-      x[p] = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
     }
   }
 
   const KvRows& out = what == 0 ? A.q_out : A.k_out;
-  if (what != 2 && out.ptr != nullptr && have) {
-    __nv_bfloat16* const dst = (__nv_bfloat16*)out.ptr + b * out.sb + n * out.sn;
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int h = g * kRows + p * kPerPass + sub;
-      if (h < heads) *reinterpret_cast<uint4*>(dst + h * out.sh + l * 8) = x[p];
-    }
-  }
-  if (what == 0 || A.data == nullptr || slot < 0) return;       // (the whole warp: one token)
-
+  __nv_bfloat16* const dst = what != 2 && out.ptr != nullptr ? (__nv_bfloat16*)out.ptr + b * out.sb + n * out.sn + l * 8 : nullptr;
   const int64_t page = slot / A.page_size;
   const int in_page = (int)(slot - page * A.page_size), t = in_page & 15;
-  uint8_t* const base = A.data + (page * A.Hkv * (A.page_size / 16) + in_page / 16) * Rec::kBytes;
-  const int64_t head_bytes = (int64_t)(A.page_size / 16) * Rec::kBytes;
+  const int head_bytes = A.page_size / 16 * Rec::kBytes;
+  uint8_t* const base = A.data + page * A.Hkv * head_bytes + in_page / 16 * Rec::kBytes;
+  const int code_at = what == 1 ? Rec::key(t, l * 8) : Rec::value(t, l * 8), scale_at = what == 1 ? Rec::key_scale(t, l >> 1) : Rec::value_scale(t, l >> 1);
+
+#pragma unroll 1
+  for (int first = h0; first < h1; first += kRows) {
+    uint4 x[kPasses];
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int h = g * kRows + p * kPerPass + sub;
-    uint32_t w[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
-    if (what == 1 && A.k_offset != nullptr && have && h < heads) {
-      const uint4 m = __ldg(reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.k_offset + h * A.D + l * 8));
-      const uint4 s = subtract_mean(x[p], m);
-      w[0] = s.x; w[1] = s.y; w[2] = s.z; w[3] = s.w;
+    for (int p = 0; p < kPasses; ++p) {
+      const int h = first + p * kPerPass + sub;
+      x[p] = make_uint4(0, 0, 0, 0);
+      if (have && h < h1) x[p] = __ldg(reinterpret_cast<const uint4*>(src + h * in.sh));
     }
-    uint32_t codes, scale;
-    quant_half_block(w, codes, scale);
-    if (h < heads) {
-      uint8_t* const rec = base + h * head_bytes;
-      *reinterpret_cast<uint32_t*>(rec + (what == 1 ? Rec::key(t, l * 8) : Rec::value(t, l * 8))) = codes;
-      if ((l & 1) == 0) rec[what == 1 ? Rec::key_scale(t, l >> 1) : Rec::value_scale(t, l >> 1)] = (uint8_t)scale;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int h = first + p * kPerPass + sub;
+      if (change) {
+        float2 f[4] = {bf16x2_to_f32(x[p].x), bf16x2_to_f32(x[p].y), bf16x2_to_f32(x[p].z), bf16x2_to_f32(x[p].w)};
+        float2 o[4];
+        if (halves) {
+          // the partner's raw words; with an odd number of quads its other half is meant
+          uint32_t a0 = x[p].x, a1 = x[p].y, b0 = x[p].z, b1 = x[p].w;
+          if (quads & 1) { a0 = x[p].z; a1 = x[p].w; b0 = x[p].x; b1 = x[p].y; }
+          o[0] = bf16x2_to_f32(__shfl_sync(0xffffffffu, a0, src_lane[0])); o[1] = bf16x2_to_f32(__shfl_sync(0xffffffffu, a1, src_lane[0]));
+          o[2] = bf16x2_to_f32(__shfl_sync(0xffffffffu, b0, src_lane[1])); o[3] = bf16x2_to_f32(__shfl_sync(0xffffffffu, b1, src_lane[1]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = make_float2(f[i].y, f[i].x);
+        }
+        float r = 1.f;
+        if (normed) {
+          float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s2 = ffma2(f[i], f[i], s2);
+          float s = s2.x + s2.y;
+#pragma unroll
+          for (int d = 1; d < kLanes; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+          r = rsqrtf(fmaf(s, A.inv_d, A.eps));
+        }
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[2 * i] = f[i].x * own[2 * i];
+          y[2 * i + 1] = f[i].y * own[2 * i + 1];
+        }
+        if (turned) {                      // (elsewhere an infinite neighbour times 0 would be NaN)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[2 * i] = fmaf(o[i].x, other[2 * i], y[2 * i]);
+            y[2 * i + 1] = fmaf(o[i].y, other[2 * i + 1], y[2 * i + 1]);
+          }
+        }
+        x[p] = make_uint4(pack_bf16(y[0] * r, y[1] * r), pack_bf16(y[2] * r, y[3] * r), pack_bf16(y[4] * r, y[5] * r), pack_bf16(y[6] * r, y[7] * r));
+      }
+      if (dst != nullptr && have && h < h1) *reinterpret_cast<uint4*>(dst + h * out.sh) = x[p];
+      if (to_cache) {
+        uint32_t w[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
+        if (what == 1 && A.k_offset != nullptr && have && h < h1) {
+          const uint4 m = __ldg(reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.k_offset + h * A.D + l * 8));
+          const uint4 s = subtract_mean(x[p], m);
+          w[0] = s.x; w[1] = s.y; w[2] = s.z; w[3] = s.w;
+        }
+        uint32_t codes, scale;
+        quant_half_block(w, codes, scale);
+        if (h < h1 && slot >= 0) {
+          uint8_t* const rec = base + (int64_t)h * head_bytes;
+          *reinterpret_cast<uint32_t*>(rec + code_at) = codes;
+          if ((l & 1) == 0) rec[scale_at] = (uint8_t)scale;
+        }
+      }
     }
   }
 }
 
-cudaError_t launch_kv_tokens(const KvTokensArgs& a, cudaStream_t stream) {
-  const int rows = a.DS == 128 ? 8 : 16;
-  const int64_t groups = (a.Hq + rows - 1) / rows + (int64_t)(a.Hkv + rows - 1) / rows * (a.v != nullptr ? 2 : 1);
-  const int64_t ctas = ((int64_t)a.B * a.N * groups + kTokenThreads / 32 - 1) / (kTokenThreads / 32);
-  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  if (a.DS == 128) kv_tokens_kernel<128><<<(int)ctas, kTokenThreads, 0, stream>>>(a);
-  else kv_tokens_kernel<64><<<(int)ctas, kTokenThreads, 0, stream>>>(a);
+cudaError_t launch_kv_tokens(KvTokensArgs a, cudaStream_t stream) {
+  int sms;
+  if (cudaError_t e = sm_count(&sms); e != cudaSuccess) return e;
+  const int rows = a.DS == 128 ? 8 : 16;                        // kRows
+  const int most = a.Hq > a.Hkv ? a.Hq : a.Hkv, tokens = a.B * a.N;
+  // as many heads per warp as leave two rounds of warps; the angles and weights of a token are then fetched once for them
+  const int64_t want = 64ll * sms;
+  a.span = rows;
+  while (a.span < most && (int64_t)tokens * ((a.Hq + 2 * a.span - 1) / (2 * a.span) + (a.Hkv + 2 * a.span - 1) / (2 * a.span)) >= want) a.span *= 2;
+  const int groups = (a.Hq + a.span - 1) / a.span + (a.Hkv + a.span - 1) / a.span * (a.v != nullptr ? 2 : 1);
+  if (groups > 65535) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)(((int64_t)tokens + kTokenThreads / 32 - 1) / (kTokenThreads / 32)), groups);
+  if (a.DS == 128) kv_tokens_kernel<128><<<grid, kTokenThreads, 0, stream>>>(a);
+  else kv_tokens_kernel<64><<<grid, kTokenThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
