@@ -171,17 +171,18 @@ struct KvTokensArgs {                     // norm, rotation, cache (kv_tokens.cu
   uint8_t* data;                          // the cache, or null
   const int64_t* slots;                   // [B * N]
   const void* k_offset;
-  int page_size;
+  int page_size, page_shift;
   int64_t num_slots;
   int span;                               // heads per warp: set by the launch
 };
 cudaError_t launch_kv_tokens(KvTokensArgs a, cudaStream_t stream);
+cudaError_t launch_kv_append(const KvTokensArgs& a, cudaStream_t stream);     // k and v [N, Hkv, D] as they are to the cache
 
 struct KvReadArgs {
   const uint8_t* data;
   const int64_t* slots;                   // [T]
   int64_t T, num_slots;
-  int Hkv, D, DS, page_size;
+  int Hkv, D, DS, page_shift;
   const void* k_offset;
   void *k, *v;                            // bf16 [T, Hkv, D]
 };

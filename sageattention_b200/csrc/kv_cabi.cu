@@ -18,6 +18,9 @@ int check_cache(const sage3_kv_cache* c) {
   return SAGE3_OK;
 }
 
+// of a page size that check_cache has let through
+inline int shift_of(int page_size) { return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7; }
+
 // rows of 16-byte vectors
 int check_rows(const sage3_tensor& t) {
   if (!aligned(t.ptr, 16) || t.stride_b % 8 || t.stride_h % 8 || t.stride_n % 8) return SAGE3_ERR_ARGUMENT;
@@ -84,10 +87,10 @@ int sage3_kv_tokens(const sage3_kv_tokens_args* a, void* stream) {
     if (a->cache->num_kv_heads != a->Hkv || a->cache->head_dim != a->D) return SAGE3_ERR_ARGUMENT;
     k.DS = a->cache->head_dim_stored;
     k.data = (uint8_t*)a->cache->data; k.slots = a->slots; k.k_offset = a->cache->k_offset;
-    k.page_size = a->cache->page_size; k.num_slots = a->cache->num_pages * a->cache->page_size;
+    k.page_size = a->cache->page_size; k.page_shift = shift_of(a->cache->page_size); k.num_slots = a->cache->num_pages * a->cache->page_size;
     k.v = a->v.ptr;
   }
-  if ((int64_t)a->B * a->N >= (1ll << 31)) return SAGE3_ERR_UNSUPPORTED;
+  if ((int64_t)a->B * a->N >= (1ll << 31) - 64 || (int64_t)a->Hq + 2ll * a->Hkv > 65535 * 8) return SAGE3_ERR_UNSUPPORTED;
   if ((int64_t)a->B * a->N == 0) return SAGE3_OK;
   k.q = rows_of(a->q); k.k = rows_of(a->k); k.vr = rows_of(a->v); k.q_out = rows_of(a->q_out); k.k_out = rows_of(a->k_out);
   k.B = a->B; k.N = a->N; k.Hq = a->Hq; k.Hkv = a->Hkv; k.D = a->D;
@@ -95,7 +98,10 @@ int sage3_kv_tokens(const sage3_kv_tokens_args* a, void* stream) {
   k.eps = a->eps; k.inv_d = 1.0f / (float)a->D;
   k.cos = a->cos; k.sin = a->sin; k.places = a->places; k.rot = a->rot_dim; k.adjacent = a->adjacent_pairs != 0;
   k.positions = a->positions; k.positions64 = a->positions_int64 != 0;
-  cudaError_t e = sage3::launch_kv_tokens(k, (cudaStream_t)stream);
+  // keys and values that only go to the cache have a kernel of their own
+  const bool as_is = a->Hq == 0 && a->B == 1 && a->k_out.ptr == nullptr && a->k_weight == nullptr && a->rot_dim == 0;
+  if (as_is && a->Hkv > 32767) return SAGE3_ERR_UNSUPPORTED;
+  cudaError_t e = as_is ? sage3::launch_kv_append(k, (cudaStream_t)stream) : sage3::launch_kv_tokens(k, (cudaStream_t)stream);
   return e == cudaSuccess ? SAGE3_OK : sage3::cuda_fail(e);
 }
 
@@ -104,10 +110,10 @@ int sage3_kv_read(const sage3_kv_cache* cache, const int64_t* slots, int64_t T, 
   if (T < 0) return SAGE3_ERR_ARGUMENT;
   if (T == 0) return SAGE3_OK;
   if (!slots || !k || !v || !aligned(k, 16) || !aligned(v, 16)) return SAGE3_ERR_ARGUMENT;
-  if (T >= (1ll << 31)) return SAGE3_ERR_UNSUPPORTED;
+  if (T >= (1ll << 31) || cache->num_kv_heads > 32767) return SAGE3_ERR_UNSUPPORTED;
   sage3::KvReadArgs a{};
   a.data = (const uint8_t*)cache->data; a.slots = slots; a.T = T; a.num_slots = cache->num_pages * cache->page_size;
-  a.Hkv = cache->num_kv_heads; a.D = cache->head_dim; a.DS = cache->head_dim_stored; a.page_size = cache->page_size;
+  a.Hkv = cache->num_kv_heads; a.D = cache->head_dim; a.DS = cache->head_dim_stored; a.page_shift = shift_of(cache->page_size);
   a.k_offset = cache->k_offset; a.k = k; a.v = v;
   cudaError_t e = sage3::launch_kv_read(a, (cudaStream_t)stream);
   return e == cudaSuccess ? SAGE3_OK : sage3::cuda_fail(e);
