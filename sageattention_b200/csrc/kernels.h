@@ -21,6 +21,18 @@ inline cudaError_t sm_count(int* sms) {
   return cudaSuccess;
 }
 
+// The kernel's dynamic shared memory, set once per device (`done`: a bit for each)
+template <class K>
+cudaError_t allow_smem(K* kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit != 0 && (done.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); e != cudaSuccess) return e;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
 // Launch; with `pdl` as a programmatic dependent of the kernel before it on the stream (the kernel then waits with
 // griddepcontrol.wait before it touches anything that one writes).
 template <class... P, class... A>

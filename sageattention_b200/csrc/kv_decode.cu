@@ -565,7 +565,8 @@ Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
 template <int D, int NB>
 cudaError_t launch(const Params& P, const Plan& p, bool split, cudaStream_t stream) {
   constexpr int smem = smem_bytes<D, NB>();
-  if (cudaError_t e = cudaFuncSetAttribute(kv_decode_kernel<D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return e;
+  static std::atomic<uint64_t> allowed;
+  if (cudaError_t e = allow_smem(kv_decode_kernel<D, NB>, smem, allowed); e != cudaSuccess) return e;
   if (cudaError_t e = launch_pdl(kv_decode_kernel<D, NB>, dim3((unsigned)p.ctas), kWarps * 32, smem, stream, false, P); e != cudaSuccess) return e;
   if (!split) return cudaGetLastError();
   const int64_t warps = (int64_t)P.a.B * P.a.Hkv * P.tiles * 8 * NB;

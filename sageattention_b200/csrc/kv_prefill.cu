@@ -684,7 +684,8 @@ cudaError_t launch(const Params2& P, const Plan2& p, cudaStream_t stream) {
     return e != cudaSuccess ? e : f.numRegs < kLaunchRegs ? cudaErrorInvalidConfiguration : cudaSuccess;
   }();
   if (regs_ok != cudaSuccess) return regs_ok;
-  if (cudaError_t e = cudaFuncSetAttribute(kv_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return e;
+  static std::atomic<uint64_t> allowed;
+  if (cudaError_t e = allow_smem(kv_prefill_kernel<D>, smem, allowed); e != cudaSuccess) return e;
   if (cudaError_t e = launch_pdl(kv_prefill_kernel<D>, dim3((unsigned)p.items, P.splits), kThreads2, smem, stream, false, P); e != cudaSuccess) return e;
   if (P.splits == 1) return cudaGetLastError();
   return launch_pdl(kv_prefill_join_kernel<D>, dim3((unsigned)(p.items * kItemRows / 8)), 256, 0, stream, true, P);

@@ -79,8 +79,11 @@ def _strides(x):
 
 
 def _run(fn, struct, device, where):
-    with _on_device(device):
+    if device.index == torch.cuda.current_device():
         st = fn(C.byref(struct), _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            st = fn(C.byref(struct), _stream_ptr(device))
     if st:
         _lib.check(st, where)
 
@@ -100,22 +103,28 @@ class FP4KVCache:
     __slots__ = ("data", "num_pages", "num_kv_heads", "page_size", "head_dim", "k_offset", "device", "_key", "_struct", "_ref")
 
     def __init__(self, data: torch.Tensor, head_dim: int, page_size: int = 64, k_offset: Optional[torch.Tensor] = None):
-        _require(page_size in _PAGE_SIZES, f"page_size must be one of {_PAGE_SIZES}")
-        _require(0 < head_dim <= 128 and head_dim % 8 == 0, f"Unsupported head_dim: {head_dim} (a multiple of 8, at most 128)")
-        _require(data.dtype == torch.uint8 and data.dim() == 3 and data.is_contiguous(), "data must be a contiguous uint8 tensor [num_pages, num_kv_heads, page_bytes]")
+        if page_size not in _PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {_PAGE_SIZES}")
+        if not (0 < head_dim <= 128 and head_dim % 8 == 0):
+            raise ValueError(f"Unsupported head_dim: {head_dim} (a multiple of 8, at most 128)")
+        if data.dtype != torch.uint8 or data.dim() != 3 or not data.is_contiguous():
+            raise ValueError("data must be a contiguous uint8 tensor [num_pages, num_kv_heads, page_bytes]")
         pages, heads, nbytes = data.shape
-        _require(nbytes == self.page_bytes(head_dim, page_size), f"pages of {page_size} tokens of head_dim {head_dim} take {self.page_bytes(head_dim, page_size)} bytes, not {nbytes}")
-        _require(pages > 0 and heads > 0, "the cache must have pages and heads")
-        _require(data.data_ptr() % 16 == 0, "data must start on a 16-byte boundary")
+        if nbytes != self.page_bytes(head_dim, page_size):
+            raise ValueError(f"pages of {page_size} tokens of head_dim {head_dim} take {self.page_bytes(head_dim, page_size)} bytes, not {nbytes}")
+        if pages == 0 or heads == 0:
+            raise ValueError("the cache must have pages and heads")
+        pointer, device, offset = data.data_ptr(), data.device, None
         if k_offset is not None:
-            _check_bf16(k_offset)
-            _check_ids("k_offset", k_offset, torch.bfloat16, (heads, head_dim), data.device)
-            _require(k_offset.data_ptr() % 16 == 0, "k_offset must start on a 16-byte boundary")
+            if k_offset.dtype != torch.bfloat16 or k_offset.shape != (heads, head_dim) or k_offset.device != device or not k_offset.is_contiguous():
+                raise ValueError(f"k_offset must be a contiguous bfloat16 tensor [{heads}, {head_dim}] on the device of data")
+            offset = k_offset.data_ptr()
+        if (pointer | (offset or 0)) & 15:
+            raise ValueError("data and k_offset must start on a 16-byte boundary")
         self.data, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim, self.k_offset = data, pages, heads, page_size, head_dim, k_offset
-        self.device = data.device
-        self._key = (pages, heads, head_dim, page_size, data.device, k_offset is None)
-        self._struct = _lib.KvCache(data.data_ptr(), pages, heads, page_size, head_dim, _stored_dim(head_dim),
-                                    None if k_offset is None else k_offset.data_ptr())
+        self.device = device
+        self._key = (pages, heads, head_dim, page_size, device, offset is None)
+        self._struct = _lib.KvCache(pointer, pages, heads, page_size, head_dim, 64 if head_dim <= 64 else 128, offset)
         self._ref = C.pointer(self._struct)
 
     @staticmethod
@@ -160,13 +169,13 @@ class FP4KVCache:
             _check_ids("slots", slots, torch.int64, slots.shape, self.device)
         dev = self.device
         _check_b200(dev, self.data)
-        kv = torch.empty((2, T, self.num_kv_heads, self.head_dim), dtype=torch.bfloat16, device=dev)
-        p = kv.data_ptr()
+        k = torch.empty((T, self.num_kv_heads, self.head_dim), dtype=torch.bfloat16, device=dev)
+        v = torch.empty_like(k)
         with _on_device(dev):
-            st = _lib.load().sage3_kv_read(self._ref, slots.data_ptr(), T, p, p + kv.nbytes // 2, _stream_ptr(dev))
+            st = _lib.load().sage3_kv_read(self._ref, slots.data_ptr(), T, k.data_ptr(), v.data_ptr(), _stream_ptr(dev))
         if st:
             _lib.check(st, "sage3_kv_read")
-        return kv.unbind()
+        return k, v
 
     def _check_tokens(self, k, v, slots):
         _check_bf16(k, v)
@@ -209,9 +218,9 @@ def build_block_tables(lens_before: torch.Tensor, lens_new: torch.Tensor, block_
     dev, a = plan.device, _lib.KvTablesArgs.from_buffer_copy(plan.struct)
     B, n = a.B, a.num_tokens
     # one allocation for all of int32
-    ints = torch.empty(2 * B + 2 + n, dtype=torch.int32, device=dev)
-    kv_lens, cu, taken, positions = ints.split((B, B + 1, 1, n))
-    slots = torch.empty(n, dtype=torch.int64, device=dev)
+    ints = lens_new.new_empty(2 * B + 2 + n)
+    kv_lens, cu, taken, positions = torch.split_with_sizes(ints, (B, B + 1, 1, n))
+    slots = lens_new.new_empty(n, dtype=torch.int64)
     p = ints.data_ptr()
     a.lens_before, a.lens_new, a.free_pages, a.block_table = lens_before.data_ptr(), lens_new.data_ptr(), free_pages.data_ptr(), block_table.data_ptr()
     a.kv_lens, a.cu_seqlens_q, a.pages_taken, a.positions, a.slots = p, p + 4 * B, p + 8 * B + 4, p + 8 * B + 8, slots.data_ptr()
@@ -307,8 +316,9 @@ def _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight):
         other |= cp | sp
         if positions is not None:
             a.positions = positions.data_ptr()
-    _check_aligned(qp | kp, "q and k")
-    _check_aligned(other, "weights, cos and sin")
+    if (qp | kp | other) & 15:
+        _check_aligned(qp | kp, "q and k")
+        _check_aligned(other, "weights, cos and sin")
 
 
 def _check_out(o, x):
@@ -341,7 +351,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
     _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight)
     yq, yk = (torch.empty_like(q), torch.empty_like(k)) if out is None else out
     if q.dim() == 3:
-        a.q_out, a.k_out = _lib.Tensor(yq.data_ptr(), 0, *_strides(yq)), _lib.Tensor(yk.data_ptr(), 0, *_strides(yk))
+        for y, t in ((yq, a.q_out), (yk, a.k_out)):
+            t.ptr = y.data_ptr()
+            t.stride_n, t.stride_h, _ = y.stride()
     else:
         a.q_out, a.k_out = (_lib.Tensor(y.data_ptr(), *_as_bhnd_strides(y, tensor_layout)[4:]) for y in (yq, yk))
     if a.B and a.N:
@@ -374,7 +386,10 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache
         out = torch.empty_like(q)
     vp = v.data_ptr()
     _check_aligned(vp, "v")
-    a.q_out, a.v.ptr, a.cache, a.slots = _lib.Tensor(out.data_ptr(), 0, *_strides(out)), vp, cache._ref, slots.data_ptr()
+    t = a.q_out
+    t.ptr = out.data_ptr()
+    t.stride_n, t.stride_h, _ = out.stride()
+    a.v.ptr, a.cache, a.slots = vp, cache._ref, slots.data_ptr()
     if a.N:
         _run(_lib.load().sage3_kv_tokens, a, plan.device, "sage3_kv_tokens")
     return out
@@ -407,9 +422,10 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
         out = torch.empty_like(q)
     lse = torch.empty(plan.rows, dtype=torch.float32, device=dev) if return_lse else None
     if a.total_q:
-        ws = torch.empty(plan.workspace, dtype=torch.uint8, device=dev)
+        ws = cache.data.new_empty(plan.workspace)
         qp = q.data_ptr()
-        _check_aligned(qp, "q")
+        if qp & 15:
+            _check_aligned(qp, "q")
         a.cache, a.q, a.out, a.kv_lens, a.block_table = cache._ref, qp, out.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr()
         a.out_stride_h, a.out_stride_n = _strides(out)
         if lse is not None:
