@@ -88,42 +88,37 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(co
     const KvSeq s(A, b);
     return A.Hkv * tiles_of<kRows>(s, P.group) * blocks_of(s);
   };
-  int total = 0;
-  for (int b = threadIdx.x; b < A.B; b += kWarps * 32) total += units(b);
+  // a thread has some sequences next to one another; one scan gives it the units in front of them, and their total
+  const int each = (A.B + kWarps * 32 - 1) / (kWarps * 32), b_first = min((int)threadIdx.x * each, A.B), b_last = min(b_first + each, A.B);
+  int mine = 0;
+  for (int b = b_first; b < b_last; ++b) mine += units(b);
+  int incl = mine;
 #pragma unroll
-  for (int d = 16; d > 0; d /= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
-  if (lane == 0) scan_s[warp] = total;
+  for (int d = 1; d < 32; d *= 2) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += x;
+  }
+  if (lane == 31) scan_s[warp] = incl;
   __syncthreads();
-  total = scan_s[0] + scan_s[1] + scan_s[2] + scan_s[3];
+  int total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += scan_s[w];
+    total += scan_s[w];
+  }
   const int per = (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x);
   int unit = blockIdx.x * per;
   const int unit_end = min(unit + per, total);
   if (blockIdx.x == 0 && threadIdx.x == 0) P.header->per = per;
   if (unit >= unit_end) return;
-  // the sequence that the first one belongs to
-  int before = 0;
-  for (int b0 = 0;; b0 += kWarps * 32) {
-    __syncthreads();
-    const int b = b0 + threadIdx.x;
-    const int mine = b < A.B ? units(b) : 0;
-    int incl = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int x = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += x;
-    }
-    if (lane == 31) scan_s[warp] = incl;
-    if (threadIdx.x == 0) where_s[0] = -1;
-    __syncthreads();
-    incl += before;
-    for (int w = 0; w < warp; ++w) incl += scan_s[w];
-    if (unit < incl && unit >= incl - mine) { where_s[0] = b; where_s[1] = incl - mine; }
-    __syncthreads();
-    if (where_s[0] >= 0 || b0 + kWarps * 32 >= A.B) break;      // (it is found: unit < total)
-    before += scan_s[0] + scan_s[1] + scan_s[2] + scan_s[3];
+  if (unit >= before && unit < before + mine) {                // one of this thread's is the first
+    int b = b_first, x = before;
+    for (int n_b; unit >= x + (n_b = units(b)); ++b) x += n_b;
+    where_s[0] = b; where_s[1] = x;
   }
-  int b = max(where_s[0], 0);
-  int rest = unit - where_s[1];        // units of sequence b before this one
+  __syncthreads();
+  int b = where_s[0];
+  int rest = unit - where_s[1];            // units of sequence b before this one
 
 #pragma unroll 1
   while (unit < unit_end) {
@@ -502,25 +497,44 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const Params P) {
   if (first == last) return;
   // the first CTA had the item last, the others had it first
   auto place = [&](int cta) { return ((int64_t)cta * 2 + (cta == first ? 1 : 0)) * kRows + row_id; };
-  float m = kLowest;
-  for (int x = first + lane; x <= last; x += 32) m = fmaxf(m, P.ml_part[place(x)].x);
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  float acc[V], l = 0.f;
+  // four parts at a time, all of them loaded before the first is used
+  constexpr int kAtOnce = 4;
+  float acc[V], l = 0.f, m = kLowest;
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int x = first; x <= last; ++x) {
-    const int64_t at = place(x);
-    const float2 ml = P.ml_part[at];
-    const float w = ex2_approx(ml.x - m);
-    l = fmaf(w, ml.y, l);
-    if constexpr (V == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(P.o_part + at * D + lane * 4);
-      acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]); acc[2] = fmaf(w, v.z, acc[2]); acc[3] = fmaf(w, v.w, acc[3]);
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(P.o_part + at * D + lane * 2);
-      acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]);
+#pragma unroll 1
+  for (int x = first; x <= last; x += kAtOnce) {
+    float2 ml[kAtOnce];
+    float v[kAtOnce][V];
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y) {
+      ml[y] = make_float2(kLowest, 0.f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[y][i] = 0.f;
+      if (x + y <= last) {
+        const int64_t at = place(x + y);
+        ml[y] = P.ml_part[at];
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          const float2 u = *reinterpret_cast<const float2*>(P.o_part + at * D + lane * V + i);
+          v[y][i] = u.x; v[y][i + 1] = u.y;
+        }
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y) top = fmaxf(top, ml[y].x);
+    const float old = ex2_approx(m - top);
+    m = top;
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] *= old;
+#pragma unroll
+    for (int y = 0; y < kAtOnce; ++y) {
+      const float w = ex2_approx(ml[y].x - m);
+      l = fmaf(w, ml[y].y, l);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(w, v[y][i], acc[i]);
     }
   }
   const int tok = row / P.group, hq = h * P.group + row - tok * P.group;
