@@ -65,14 +65,13 @@ constexpr int smem_bytes() {
 }
 
 // CTAs per SM that the registers are held to
-template <int D, int NB>
-constexpr int kCtas = NB == 1 ? 4 : 3;
+constexpr int ctas_per_sm(int D, int NB) { return NB == 1 ? 4 : NB == 2 ? 3 : D == 64 && NB == 3 ? 3 : 2; }
 
 // The work: an item is a (sequence, kv head, tile of rows), a unit one of its blocks of 128 keys.  All units, in this order, are dealt out in
 // equal runs, so that ragged batches and single long sequences fill the chip alike; a CTA's run may end inside an item and go on to
 // others.  Only its first and its last item can be shared with other CTAs: two places for partial results each.
 template <int D, int NB>                  // stored head dim, 8-row blocks
-__global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(const Params P) {
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_kernel(const Params P) {
   using Rec = KvRecord<D>;
   constexpr int kRows = 8 * NB, kRecs = kChunk / 16, kStageBytes = kRecs * Rec::kBytes;
   constexpr int kKS = D / 16;             // k steps of the scores = tiles of 16 channels of the output
@@ -432,9 +431,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(co
       }
     }
     __syncthreads();
-    constexpr int kPer = kRows * D / (kWarps * 32);                       // channels of a row per thread
-    const int row = threadIdx.x / (D / kPer), ch = threadIdx.x % (D / kPer) * kPer;
-    if (row0 + row < rows) {
+    constexpr int kPer = D / 32;                                          // channels of a row per lane; a warp has every fourth row
+#pragma unroll 1
+    for (int row = warp; row < kRows && row0 + row < rows; row += kWarps) {
       float m = kLowest, l = 0.f, wgt[kWarps];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml_s[w * kRows + row].x);
@@ -450,25 +449,24 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, NB>) kv_decode_kernel(co
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) acc[k] = fmaf(wgt[w], o_s[(w * kRows + row) * (D + 4) + ch + k], acc[k]);
+        for (int k = 0; k < kPer; k += 2) {
+          const float2 x = *reinterpret_cast<const float2*>(o_s + (w * kRows + row) * (D + 4) + lane * kPer + k);
+          acc[k] = fmaf(wgt[w], x.x, acc[k]); acc[k + 1] = fmaf(wgt[w], x.y, acc[k + 1]);
+        }
       const int tok = (row0 + row) / P.group, hq = h * P.group + row0 + row - tok * P.group;
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh;
+        __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh + lane * kPer;
+        if (lane * kPer < A.D)
 #pragma unroll
-        for (int k = 0; k < kPer; k += 4)
-          if (ch + k < A.D)
-            *reinterpret_cast<uint2*>(out + ch + k) =
-                make_uint2(pack_bf16(acc[k] * inv, acc[k + 1] * inv), pack_bf16(acc[k + 2] * inv, acc[k + 3] * inv));
-        if (ch == 0 && A.lse != nullptr)
-          A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, add_s[row]);
+          for (int k = 0; k < kPer; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pack_bf16(acc[k] * inv, acc[k + 1] * inv);
+        if (lane == 0 && A.lse != nullptr) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, add_s[row]);
       } else {
         const int64_t at = ((int64_t)blockIdx.x * 2 + (head_of_item ? 1 : 0)) * kRows + row;
 #pragma unroll
-        for (int k = 0; k < kPer; k += 4)
-          *reinterpret_cast<float4*>(P.o_part + at * D + ch + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
-        if (ch == 0) P.ml_part[at] = make_float2(m, l);
-        if (ch == 0 && head_of_item && A.lse != nullptr) P.lse_add[((int64_t)bh * P.tiles + tile) * kRows + row] = add_s[row];
+        for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(P.o_part + at * D + lane * kPer + k) = make_float2(acc[k], acc[k + 1]);
+        if (lane == 0) P.ml_part[at] = make_float2(m, l);
+        if (lane == 0 && head_of_item && A.lse != nullptr) P.lse_add[((int64_t)bh * P.tiles + tile) * kRows + row] = add_s[row];
       }
     }
     if (head_of_item && threadIdx.x == 0) P.item_start[(int64_t)bh * P.tiles + tile] = unit;
@@ -557,14 +555,14 @@ struct Plan {
   size_t bytes;
 };
 
-// 16 rows at a time where there are more than 8; as many CTAs as fit on the chip at once, or as there are units.
+// Up to 24 (D=64: 32) rows at a time, in tiles as equal as can be; as many CTAs as fit on the chip at once, or as there are units.
 Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
   Plan p;
-  const int64_t rows = (int64_t)max_q * (Hq / Hkv);
-  p.nb = rows <= 8 ? 1 : 2;
-  p.tiles = (int)((rows + 8 * p.nb - 1) / (8 * p.nb));
+  const int64_t rows = (int64_t)max_q * (Hq / Hkv), most = DS == 64 ? 32 : 24;
+  p.tiles = (int)((rows + most - 1) / most);
+  p.nb = (int)((rows + 8 * p.tiles - 1) / (8 * p.tiles));
   const int64_t items = (int64_t)B * Hkv * p.tiles, blocks = ((int64_t)max_k + kBlock - 1) / kBlock;
-  const int64_t fit = (int64_t)sms * (p.nb == 1 ? 4 : 3);
+  const int64_t fit = (int64_t)sms * ctas_per_sm(DS, p.nb);
   p.units = items * blocks;
   p.rows = items * 8 * p.nb;
   p.ctas = p.units < fit ? p.units : fit;
@@ -612,8 +610,11 @@ cudaError_t launch_kv_decode(const KvAttnArgs& a, cudaStream_t stream) {
   P.item_start = (int*)(w + p.starts); P.lse_add = (float*)(w + p.adds);
   P.ml_part = (float2*)(w + p.ml); P.o_part = (float*)(w + p.o);
   const bool split = a.max_k > kBlock;     // else an item is one unit
-  if (a.DS == 128) return p.nb == 1 ? launch<128, 1>(P, p, split, stream) : launch<128, 2>(P, p, split, stream);
-  return p.nb == 1 ? launch<64, 1>(P, p, split, stream) : launch<64, 2>(P, p, split, stream);
+  if (a.DS == 128) return p.nb == 1 ? launch<128, 1>(P, p, split, stream) : p.nb == 2 ? launch<128, 2>(P, p, split, stream) : launch<128, 3>(P, p, split, stream);
+  return p.nb == 1   ? launch<64, 1>(P, p, split, stream)
+         : p.nb == 2 ? launch<64, 2>(P, p, split, stream)
+         : p.nb == 3 ? launch<64, 3>(P, p, split, stream)
+                     : launch<64, 4>(P, p, split, stream);
 }
 
 }  // namespace sage3
