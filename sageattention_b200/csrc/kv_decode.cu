@@ -27,6 +27,7 @@ struct Header {                           // at the front of the workspace, for 
 struct Params {
   KvAttnArgs a;
   int group, tiles, page_shift;           // query heads per kv head; tiles of rows of the longest sequence
+  uint32_t group_inverse;                 // 2^32 / group rounded up: exact for quotients of the few rows there are
   float scale_log2;
   Header* header;
   int* item_start;                        // [B * Hkv, tiles]: number of the item's first unit
@@ -82,6 +83,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   pdl_launch_dependents();
 
+  auto group_of = [&](int row) { return P.group == 1 ? row : (int)__umulhi((uint32_t)row, P.group_inverse); };       // row / group
+
   // ---- this CTA's units
   auto units = [&](int b) {
     const KvSeq s(A, b);
@@ -132,9 +135,22 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
     const int h = item / tiles, tile = item - h * tiles, bh = b * A.Hkv + h;
     const int rows = seq.q_len * P.group, row0 = tile * kRows;
     const int last_row = min(rows, row0 + kRows) - 1;
-    const int see_all = seq.seen(A, row0 / P.group), see_any = seq.seen(A, last_row / P.group);   // keys that each row, that any row sees
+    const int see_all = seq.seen(A, group_of(row0)), see_any = seq.seen(A, group_of(last_row));   // keys that each row, that any row sees
     const int begin = block * kBlock, end = min(begin + take * kBlock, see_any);
     const bool whole = take == blocks, head_of_item = block == 0;
+
+    // ---- queries under way: this lane the channels c D/4 ... of row n of each block (used when keys have been asked for: both take as long)
+    uint4 q_raw[NB][D / 32];
+#pragma unroll
+    for (int r = 0; r < NB; ++r) {
+      const int row = row0 + r * 8 + n, tok = group_of(row), hq = h * P.group + row - tok * P.group;
+      const uint4* const src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.q + (int64_t)(seq.q0 + tok) * A.q_sn + hq * A.q_sh + c * (D / 4));
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        q_raw[r][i] = make_uint4(0, 0, 0, 0);
+        if (row < rows && c * (D / 4) + i * 8 < A.D) q_raw[r][i] = __ldg(src + i);
+      }
+    }
 
     // ---- keys on their way: chunk number `i` of this warp is keys begin + 32 (kWarps i + warp) ...
     const uint32_t ring = smem_u32(sm) + warp * (kStages * kStageBytes);
@@ -184,19 +200,16 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) fetch(i);
 
-    // ---- queries: B fragments, this lane the channels c D/4 ... of row n of each block
+    // ---- queries: B fragments
     uint32_t qf[NB][kKS][2];
     float factor[NB][2];                   // of the scores of rows 2 c, 2 c + 1: softmax scale times what undoes the row's power of two
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
-      const int row = row0 + r * 8 + n, tok = row / P.group, hq = h * P.group + row - tok * P.group;
-      const __nv_bfloat16* const src = (const __nv_bfloat16*)A.q + (int64_t)(seq.q0 + tok) * A.q_sn + hq * A.q_sh + c * (D / 4);
       uint32_t w[D / 8];
       uint32_t m2 = 0;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row < rows && c * (D / 4) + i * 8 < A.D) x = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        const uint4 x = q_raw[r][i];
         w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
         m2 = habsmax2(m2, habsmax2(habsmax2(x.x, x.y), habsmax2(x.z, x.w)));
       }
@@ -238,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = row0 + r * 8 + 2 * c + j;
-        limit[r][j] = row < rows ? seq.seen(A, row / P.group) : 0;
+        limit[r][j] = row < rows ? seq.seen(A, group_of(row)) : 0;
       }
 
     float o[kKS][NB][4];
@@ -453,7 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
           const float2 x = *reinterpret_cast<const float2*>(o_s + (w * kRows + row) * (D + 4) + lane * kPer + k);
           acc[k] = fmaf(wgt[w], x.x, acc[k]); acc[k + 1] = fmaf(wgt[w], x.y, acc[k + 1]);
         }
-      const int tok = (row0 + row) / P.group, hq = h * P.group + row0 + row - tok * P.group;
+      const int tok = group_of(row0 + row), hq = h * P.group + row0 + row - tok * P.group;
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh + lane * kPer;
@@ -602,6 +615,7 @@ cudaError_t launch_kv_decode(const KvAttnArgs& a, cudaStream_t stream) {
   Params P;
   P.a = a;
   P.group = a.Hq / a.Hkv; P.tiles = p.tiles;
+  P.group_inverse = (uint32_t)(0xffffffffu / (uint32_t)P.group) + 1;
   P.scale_log2 = a.sm_scale * kLog2e;
   P.page_shift = 0;
   while ((1 << P.page_shift) < a.page_size) ++P.page_shift;
