@@ -12,8 +12,7 @@ captured into a CUDA graph.  The reference has no counterpart: its operators kee
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -46,10 +45,19 @@ def _check_aligned(pointers, what):
         raise ValueError(f"{what} must start on a 16-byte boundary")
 
 
-# What a call with given shapes, strides, types and options needs is worked out once, as for the other operators (api.py): the checks and
-# the argument struct but for its pointers.  A call looks its plan up by all of these, copies the struct and fills the pointers in.
+# What a call with given sizes and options needs is worked out once, as for the other operators (api.py): the checks and the argument struct
+# but for its pointers.  A call looks its plan up by these, copies the struct and fills the pointers in.  Tensors of which only one
+# shape, type and layout will do are not part of what a plan is found by, but looked at (_is) in every call; where one is not as it should
+# be, the checks of the plan are run again to say so.  (Looking a tensor up costs 1.1 us, looking at it 0.45.)
 class _Plan:
-    __slots__ = ("device", "struct", "workspace", "rows")
+    __slots__ = ("device", "struct", "workspace", "rows", "where")
+
+
+def _is(t, dtype, shape, device):
+    return t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _check_ids(name, t, dtype, shape, device):
@@ -79,7 +87,7 @@ def _strides(x):
 
 
 def _run(fn, struct, device, where):
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():           # (a tensor is on it, so CUDA is up)
         st = fn(C.byref(struct), _stream_ptr(device))
     else:
         with torch.cuda.device(device):
@@ -143,15 +151,15 @@ class FP4KVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Writes k, v (bf16 ``[T, num_kv_heads, head_dim]``) to the slots (int64 ``[T]``) ``page * page_size + place``.  Slots outside the cache
         (-1) are skipped; a slot named twice ends up with a mixture of its tokens."""
-        key = ("kv_append", k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, slots.shape, slots.stride(), slots.dtype,
-               slots.device, self._key)
+        key = ("kv_append", _sig(k), _sig(v), self._key)
         plan = _plans.get(key)
-        if plan is None:
+        if plan is None or not _is(slots, torch.int64, plan.rows, self.device):
             T = self._check_tokens(k, v, slots)
             plan = _Plan()
             a = plan.struct = _lib.KvTokensArgs()
             a.B, a.N, a.Hq, a.Hkv, a.D = 1, T, 0, self.num_kv_heads, self.head_dim
             a.k, a.v = _lib.Tensor(None, 0, *_strides(k)), _lib.Tensor(None, 0, *_strides(v))
+            plan.rows = k.shape[:1]
             _keep_plan(key, plan)
         kp, vp = k.data_ptr(), v.data_ptr()
         _check_aligned(kp | vp, "k and v")
@@ -188,8 +196,7 @@ class FP4KVCache:
         return k.shape[0]
 
 
-@dataclass
-class BlockTables:
+class BlockTables(NamedTuple):
     """What :func:`build_block_tables` gives: ``kv_lens`` int32 [B] (lengths after the step), ``cu_seqlens_q`` int32 [B+1], ``positions`` int32
     [num_tokens], ``slots`` int64 [num_tokens], ``pages_taken`` int32 [1]."""
     kv_lens: torch.Tensor
@@ -209,11 +216,10 @@ def build_block_tables(lens_before: torch.Tensor, lens_new: torch.Tensor, block_
     entries ``positions`` and ``slots`` get, the sum of ``lens_new`` or more (a padded batch); behind the last token slots are -1 and
     positions 0.  Nothing is read back: where the free pages or the columns do not suffice, table entries and slots are -1, and
     ``pages_taken`` says how many pages the step wanted."""
-    key = ("kv_tables", lens_before.shape, lens_before.stride(), lens_before.dtype, lens_before.device, lens_new.shape, lens_new.stride(), lens_new.dtype,
-           lens_new.device, free_pages.shape, free_pages.stride(), free_pages.dtype, free_pages.device, block_table.shape, block_table.stride(),
-           block_table.dtype, block_table.device, page_size, num_tokens)
+    key = ("kv_tables", _sig(lens_before), free_pages.shape, block_table.shape, block_table.stride(), page_size, num_tokens)
     plan = _plans.get(key)
-    if plan is None:
+    if (plan is None or not _is(lens_new, torch.int32, plan.where, plan.device) or not _is(free_pages, torch.int32, plan.rows, plan.device) or
+            block_table.dtype is not torch.int32 or block_table.device != plan.device):
         plan = _keep_plan(key, _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_tokens))
     dev, a = plan.device, _lib.KvTablesArgs.from_buffer_copy(plan.struct)
     B, n = a.B, a.num_tokens
@@ -241,7 +247,7 @@ def _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_
     _check_table(block_table, B, dev)
     _check_device(lens_before)
     plan = _Plan()
-    plan.device = dev
+    plan.device, plan.where, plan.rows = dev, lens_before.shape, free_pages.shape
     a = plan.struct = _lib.KvTablesArgs()
     a.row_stride, a.B, a.columns, a.num_free, a.page_size, a.num_tokens = (
         max(block_table.stride(0), block_table.shape[1]), B, block_table.shape[1], free_pages.shape[0], page_size, int(num_tokens))
@@ -277,7 +283,7 @@ def _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent
     _require(q.device == k.device, "q and k must be on one device")
     _check_rows(q, k)
     plan = _Plan()
-    plan.device = q.device
+    plan.device, plan.where, plan.rows = q.device, torch.Size(where), torch.Size((D,))
     a = plan.struct = _lib.KvTokensArgs()
     a.B, a.N, a.Hq, a.Hkv, a.D = B, N, Hq, Hkv, D
     a.q, a.k = _lib.Tensor(None, *qs), _lib.Tensor(None, *ks)
@@ -300,6 +306,25 @@ def _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent
             a.positions_int64 = int(positions.dtype == torch.int64)
     _check_device(q)
     return plan
+
+
+def _norm_rope_key(name, q, k, cos, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout, *more):
+    return (name, q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, None if cos is None else cos.shape,
+            None if cos is None or positions is None else positions.dtype, q_weight is None, k_weight is None, eps, adjacent_pairs, tensor_layout, more)
+
+
+def _norm_rope_fits(plan, cos, sin, positions, q_weight, k_weight):
+    """Whether the tensors that a plan is not found by are as it has them."""
+    dev = plan.device
+    if cos is None:
+        if sin is not None:
+            return False
+    elif sin is None or not _is(cos, torch.float32, cos.shape, dev) or not _is(sin, torch.float32, cos.shape, dev):
+        return False
+    elif positions is not None and not _is(positions, positions.dtype, plan.where, dev):
+        return False
+    return ((q_weight is None or _is(q_weight, torch.bfloat16, plan.rows, dev)) and
+            (k_weight is None or _is(k_weight, torch.bfloat16, plan.rows, dev)))
 
 
 def _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight):
@@ -343,9 +368,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
     if out is not None:
         _check_out(out[0], q)
         _check_out(out[1], k)
-    key = ("qk_norm_rope", _sig(q), _sig(k), _sig(cos), _sig(sin), _sig(positions), _sig(q_weight), _sig(k_weight), eps, adjacent_pairs, tensor_layout)
+    key = _norm_rope_key("qk_norm_rope", q, k, cos, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout)
     plan = _plans.get(key)
-    if plan is None:
+    if plan is None or not _norm_rope_fits(plan, cos, sin, positions, q_weight, k_weight):
         plan = _keep_plan(key, _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout))
     a = _lib.KvTokensArgs.from_buffer_copy(plan.struct)
     _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight)
@@ -370,10 +395,10 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache
     (the same bits as :meth:`FP4KVCache.append` of its result).  Returns the queries."""
     if out is not None:
         _check_out(out, q)
-    key = ("qk_norm_rope_append", _sig(q), _sig(k), _sig(v), _sig(slots), _sig(cos), _sig(sin), _sig(positions), _sig(q_weight), _sig(k_weight), eps,
-           adjacent_pairs, cache._key)
+    key = _norm_rope_key("qk_norm_rope_append", q, k, cos, positions, q_weight, k_weight, eps, adjacent_pairs, None, v.shape, v.stride(), v.dtype,
+                         v.device, cache._key)
     plan = _plans.get(key)
-    if plan is None:
+    if plan is None or not _is(slots, torch.int64, plan.where, plan.device) or not _norm_rope_fits(plan, cos, sin, positions, q_weight, k_weight):
         _require(q.dim() == 3, "q must be [tokens, heads, head_dim]")
         plan = _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, "NHD")
         cache._check_tokens(k, v, slots)
@@ -413,9 +438,11 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where one of their bounded waits gave up."""
     if out is not None:
         _check_out(out, q)
-    key = ("kvcache", _sig(q), cache._key, _sig(block_table), _sig(kv_lens), _sig(cu_seqlens_q), max_seqlen_q, max_seqlen_k, bool(is_causal), sm_scale)
+    key = ("kvcache", q.shape, q.stride(), q.dtype, q.device, cache._key, block_table.shape, block_table.stride(), kv_lens.shape, cu_seqlens_q is None,
+           max_seqlen_q, max_seqlen_k, bool(is_causal), sm_scale)
     plan = _plans.get(key)
-    if plan is None:
+    if (plan is None or not _is(kv_lens, torch.int32, kv_lens.shape, plan.device) or block_table.dtype is not torch.int32 or
+            block_table.device != plan.device or not (cu_seqlens_q is None or _is(cu_seqlens_q, torch.int32, plan.where, plan.device))):
         plan = _keep_plan(key, _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, is_causal, sm_scale))
     dev, a = plan.device, _lib.KvAttentionArgs.from_buffer_copy(plan.struct)
     if out is None:
@@ -467,7 +494,7 @@ def _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, 
     _check_rows(q)
     _check_device(q)
     plan = _Plan()
-    plan.device, plan.rows = dev, (T, Hq)
+    plan.device, plan.rows, plan.where = dev, (T, Hq), torch.Size((B + 1,))
     a = plan.struct = _lib.KvAttentionArgs()
     a.B, a.Hq, a.max_seqlen_q, a.max_seqlen_k, a.total_q = B, Hq, int(max_seqlen_q), max_seqlen_k, T
     a.q_stride_h, a.q_stride_n = _strides(q)

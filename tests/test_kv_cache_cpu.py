@@ -249,3 +249,39 @@ def test_c_entry_points_check_arguments():
         setattr(t, n, x)
         assert lib.sage3_kv_block_tables(C.byref(t), None) == want, n
         setattr(t, n, keep)
+
+
+def test_a_kept_plan_does_not_let_another_tensor_through(monkeypatch):
+    """Types, shapes and layouts are looked at in every call, also where an earlier one with the same sizes was right."""
+    from sageattention_b200 import kv_cache
+    calls = []
+    monkeypatch.setattr(kv_cache, "_check_device", lambda t: None)
+    monkeypatch.setattr(kv_cache, "_run", lambda fn, struct, device, where: calls.append(where))
+    monkeypatch.setattr(kv_cache, "_plans", {})
+    monkeypatch.setattr(kv_cache, "_keep_plan", lambda key, plan: kv_cache._plans.setdefault(key, plan))
+    c = cache()
+    slots = ints(0, 1, 2, dtype=torch.int64)
+    good = rope_args(positions=ints(0, 1, 2), q_weight=torch.ones(64, dtype=BF), k_weight=torch.ones(64, dtype=BF))
+    bad = [dict(cos=torch.ones(8, 32, dtype=torch.float64)), dict(sin=torch.zeros(8, 64)[:, ::2]), dict(sin=None), dict(positions=ints(0, 1)),
+           dict(positions=torch.zeros(6, dtype=torch.int32)[::2]), dict(q_weight=torch.ones(64)), dict(k_weight=torch.ones(128, dtype=BF)[::2]),
+           dict(k_weight=torch.ones(32, dtype=BF))]
+    sa.qk_norm_rope(**good)
+    sa.qk_norm_rope_append(v=tokens(), cache=c, slots=slots, **good)
+    c.append(tokens(), tokens(), slots)
+    sa.build_block_tables(**table_args())
+    assert len(calls) == 4
+    for kw in bad:
+        with pytest.raises(ValueError):
+            sa.qk_norm_rope(**{**good, **kw})
+        with pytest.raises(ValueError):
+            sa.qk_norm_rope_append(v=tokens(), cache=c, slots=slots, **{**good, **kw})
+    for s in (slots.int(), ints(0, 1, dtype=torch.int64), torch.zeros(6, dtype=torch.int64)[::2]):
+        with pytest.raises(ValueError, match="slots"):
+            sa.qk_norm_rope_append(v=tokens(), cache=c, slots=s, **good)
+        with pytest.raises(ValueError, match="slots"):
+            c.append(tokens(), tokens(), s)
+    for kw in (dict(lens_new=ints(1, 1, dtype=torch.int64)), dict(lens_new=ints(1)), dict(free_pages=torch.zeros(4, dtype=torch.int32)[::2]),
+               dict(block_table=torch.zeros(2, 4))):
+        with pytest.raises(ValueError):
+            sa.build_block_tables(**table_args(**kw))
+    assert len(calls) == 4

@@ -507,3 +507,41 @@ def test_two_calls_at_once():
             got.append(sa.sageattn_kvcache(q, cache, table, lens))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got)
+
+
+def test_a_kept_attention_plan_does_not_let_another_tensor_through():
+    g = gen(41)
+    cache, table = make_cache(g, [40, 30], 1, 64, 16)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    q, table, lens, cu = normal(g, 2, 2, 64).to(DEV), table.to(DEV), torch.tensor([40, 30], **i32), torch.tensor([0, 1, 2], **i32)
+    want = sa.sageattn_kvcache(q, cache, table, lens, cu)
+    assert torch.equal(sa.sageattn_kvcache(q, cache, table, lens), want)
+    for kw in (dict(kv_lens=lens.long()), dict(kv_lens=lens.cpu()), dict(kv_lens=torch.zeros(4, **i32)[::2]), dict(cu_seqlens_q=cu.long()),
+               dict(cu_seqlens_q=cu[:2]), dict(block_table=table.float()), dict(block_table=table.cpu())):
+        with pytest.raises(ValueError):
+            sa.sageattn_kvcache(**{**dict(q=q, cache=cache, block_table=table, kv_lens=lens, cu_seqlens_q=cu), **kw})
+
+
+@pytest.mark.parametrize("tokens", [3, 70])
+def test_nan_and_infinite_queries_stay_in_their_rows(tokens):
+    g = gen(43)
+    cache, table = make_cache(g, [300], 1, 128, 32)
+    q = normal(g, tokens, 4, 128)
+    bad = q.clone()
+    bad[1, 2, 5], bad[2, 0, 100], bad[tokens - 1, 3] = float("nan"), float("inf"), float("-inf")
+    i32 = dict(dtype=torch.int32, device=DEV)
+    args = (cache, table.to(DEV), torch.tensor([300], **i32), torch.tensor([0, tokens], **i32), tokens)
+    (a, al), (b, bl) = (sa.sageattn_kvcache(x.to(DEV), *args, return_lse=True) for x in (q, bad))
+    hit = torch.zeros(tokens, 4, dtype=torch.bool)
+    hit[1, 2] = hit[2, 0] = hit[tokens - 1, 3] = True
+    assert a.isfinite().all() and b.cpu()[hit].isnan().all() and bl.cpu()[hit].isnan().all()
+    want, _, tol, _ = R.attend(q, cache.data.cpu().numpy(), 128, 32, table.tolist(), [300], [tokens])
+    off = np.abs(b.double().cpu().numpy() - want)[~hit.numpy()]
+    assert (off <= tol[~hit.numpy()]).all()
+
+
+def test_block_tables_without_free_pages_or_tokens():
+    t, r = run_tables([5, 16], [3, 2], [[4, -1], [7, -1]], [], 16, 5)
+    assert t.tolist() == [[4, -1], [7, -1]] and r.slots.tolist() == [69, 70, 71, -1, -1] and r.pages_taken.tolist() == [1]
+    t, r = run_tables([5, 16], [0, 0], [[4, -1], [7, -1]], [], 16, 0)
+    assert r.slots.numel() == r.positions.numel() == 0 and r.kv_lens.tolist() == [5, 16] and r.cu_seqlens_q.tolist() == [0, 0, 0]
