@@ -305,7 +305,17 @@ def _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent
             _check_ids("positions", positions, positions.dtype, where, q.device)
             a.positions_int64 = int(positions.dtype == torch.int64)
     _check_device(q)
+    for x, name in ((q, "q_out"), (k, "k_out")):
+        y = _rows(torch.empty_like(x, device="meta"), tensor_layout)
+        y.ptr = None
+        setattr(a, name, y)
     return plan
+
+
+def _rows(x, tensor_layout):
+    if x.dim() == 3:
+        return _lib.Tensor(x.data_ptr(), 0, *_strides(x))
+    return _lib.Tensor(x.data_ptr(), *_as_bhnd_strides(x, tensor_layout)[4:])
 
 
 def _norm_rope_key(name, q, k, cos, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout, *more):
@@ -374,13 +384,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
         plan = _keep_plan(key, _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout))
     a = _lib.KvTokensArgs.from_buffer_copy(plan.struct)
     _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight)
-    yq, yk = (torch.empty_like(q), torch.empty_like(k)) if out is None else out
-    if q.dim() == 3:
-        for y, t in ((yq, a.q_out), (yk, a.k_out)):
-            t.ptr = y.data_ptr()
-            t.stride_n, t.stride_h, _ = y.stride()
+    if out is None:
+        yq, yk = torch.empty_like(q), torch.empty_like(k)
+        a.q_out.ptr, a.k_out.ptr = yq.data_ptr(), yk.data_ptr()      # (whose strides the plan has)
     else:
-        a.q_out, a.k_out = (_lib.Tensor(y.data_ptr(), *_as_bhnd_strides(y, tensor_layout)[4:]) for y in (yq, yk))
+        yq, yk = out
+        a.q_out, a.k_out = _rows(yq, tensor_layout), _rows(yk, tensor_layout)
     if a.B and a.N:
         _run(_lib.load().sage3_kv_tokens, a, plan.device, "sage3_kv_tokens")
     return yq, yk
@@ -403,17 +412,19 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache
         plan = _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, "NHD")
         cache._check_tokens(k, v, slots)
         _require(q.device == cache.device, "q and the cache must be on one device")
+        plan.struct.k_out = _lib.Tensor()                            # (keys go to the cache alone)
         plan.struct.v = _lib.Tensor(None, 0, *_strides(v))
         _keep_plan(key, plan)
     a = _lib.KvTokensArgs.from_buffer_copy(plan.struct)
     _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight)
     if out is None:
         out = torch.empty_like(q)
+        a.q_out.ptr = out.data_ptr()
+    else:
+        a.q_out = _rows(out, "NHD")
     vp = v.data_ptr()
-    _check_aligned(vp, "v")
-    t = a.q_out
-    t.ptr = out.data_ptr()
-    t.stride_n, t.stride_h, _ = out.stride()
+    if vp & 15:
+        _check_aligned(vp, "v")
     a.v.ptr, a.cache, a.slots = vp, cache._ref, slots.data_ptr()
     if a.N:
         _run(_lib.load().sage3_kv_tokens, a, plan.device, "sage3_kv_tokens")
@@ -446,7 +457,9 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
         plan = _keep_plan(key, _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, is_causal, sm_scale))
     dev, a = plan.device, _lib.KvAttentionArgs.from_buffer_copy(plan.struct)
     if out is None:
-        out = torch.empty_like(q)
+        out = torch.empty_like(q)                                    # (whose strides the plan has)
+    else:
+        a.out_stride_h, a.out_stride_n = _strides(out)
     lse = torch.empty(plan.rows, dtype=torch.float32, device=dev) if return_lse else None
     if a.total_q:
         ws = cache.data.new_empty(plan.workspace)
@@ -454,7 +467,6 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
         if qp & 15:
             _check_aligned(qp, "q")
         a.cache, a.q, a.out, a.kv_lens, a.block_table = cache._ref, qp, out.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr()
-        a.out_stride_h, a.out_stride_n = _strides(out)
         if lse is not None:
             a.lse = lse.data_ptr()
         if cu_seqlens_q is not None:
@@ -498,6 +510,7 @@ def _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, 
     a = plan.struct = _lib.KvAttentionArgs()
     a.B, a.Hq, a.max_seqlen_q, a.max_seqlen_k, a.total_q = B, Hq, int(max_seqlen_q), max_seqlen_k, T
     a.q_stride_h, a.q_stride_n = _strides(q)
+    a.out_stride_h, a.out_stride_n = _strides(torch.empty_like(q, device="meta"))
     a.row_stride, a.columns, a.is_causal = block_table.stride(0), block_table.shape[1], int(bool(is_causal))
     a.sm_scale = 0.0 if sm_scale is None else float(sm_scale)
     # the size of the workspace goes by the sizes alone; a pointer says whether there are offsets
