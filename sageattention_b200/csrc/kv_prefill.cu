@@ -27,10 +27,10 @@ namespace sage3 {
 
 namespace {
 
-constexpr int kThreads2 = 640, kM = 128, kN = 128, kItemRows = 2 * kM;
-// Register hand-over (setmaxnreg) moves registers inside the pool the CTA was launched with, 96 a thread; launch() checks that.
-constexpr int kLaunchRegs = 96, kSoftmaxRegs = 136, kFillRegs = 72, kRoleRegs = 56;
-static_assert(256 * kSoftmaxRegs + 256 * kFillRegs + 128 * kRoleRegs <= kThreads2 * kLaunchRegs, "setmaxnreg split exceeds the CTA's register pool");
+constexpr int kThreads2 = 512, kM = 128, kN = 128, kItemRows = 2 * kM;
+// Register hand-over (setmaxnreg) moves registers inside the pool the CTA was launched with, 128 a thread; launch() checks that.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kFillRegs = 80, kRoleRegs = 48;
+static_assert(256 * kSoftmaxRegs + 128 * (kFillRegs + kRoleRegs) <= kThreads2 * kLaunchRegs, "setmaxnreg split exceeds the CTA's register pool");
 
 template <int v>
 struct Int {
@@ -46,8 +46,8 @@ struct Lay {                              // shared memory
   // 16 bytes: channels 8 chunk ... of a row
   static __device__ __forceinline__ int at(int row, int chunk) { return (chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 };
-struct Bar {                              // byte offsets in the barrier block, of two each but for p_full and the last
-  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, p_full = 96 /* [half][tile] */, pv_half = 128, pv_done = 144, drain = 160, raw_full = 168, raw_empty = 176, tmem = 184, abort = 192, there = 196;
+struct Bar {                              // byte offsets in the barrier block, of two each but for the last
+  static constexpr int k_full = 0, k_empty = 16, v_full = 32, v_empty = 48, q_full = 64, s_full = 80, s_free = 96, p_full = 112, pv_done = 128, drain = 160, raw_full = 168, raw_empty = 176, tmem = 184, abort = 192, there = 196;
 };
 
 struct Params2 {
@@ -128,6 +128,8 @@ template <int D>
 __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 P) {
   using Rec = KvRecord<D>;
   using L = Lay<D>;
+  constexpr int kSBufs = D == 64 ? 2 : 1;
+  constexpr uint32_t kTmS = 2 * D, kTmP = 384;
   extern __shared__ uint8_t raw[];
   const KvAttnArgs& A = P.a;
   uint8_t* const smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -161,18 +163,17 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       mbar_init(bars + Bar::v_empty + 8 * i, 1);
       mbar_init(bars + Bar::q_full + 8 * i, 4);
       mbar_init(bars + Bar::s_full + 8 * i, 1);
+      mbar_init(bars + Bar::s_free + 8 * i, 4);
       mbar_init(bars + Bar::p_full + 8 * i, 4);
-      mbar_init(bars + Bar::p_full + 16 + 8 * i, 4);
-      mbar_init(bars + Bar::pv_half + 8 * i, 1);
       mbar_init(bars + Bar::pv_done + 8 * i, 1);
     }
     mbar_init(bars + Bar::drain, 1);
     mbar_init(bars + Bar::raw_full, 1);
-    mbar_init(bars + Bar::raw_empty, 8);
+    mbar_init(bars + Bar::raw_empty, 4);
     *abort_s = 0;
     fence_mbar_init();
   }
-  if (warp == 16) {
+  if (warp == 12) {
     tmem_alloc(bars + Bar::tmem, 512);
     tmem_relinquish();
   }
@@ -182,88 +183,63 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::bars + Bar::tmem);
   int fail = 0;
 
-  if (warp >= 16) {
+  if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
-    if (warp == 16) {
+    if (warp == 12) {
       // ---------------------------------------------------------------- MMA
       constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);                     // 8-row groups, version, 128-byte swizzle
       constexpr uint32_t idesc_s = idesc_f16(kN, false), idesc_o = idesc_f16(D, true);
       const uint32_t q_lo = ((base + L::q) >> 4) | (1u << 16), k_lo = ((base + L::k) >> 4) | (1u << 16);
       const uint32_t v_lo = ((base + L::v) >> 4) | ((uint32_t)(L::kHalf >> 4) << 16);     // leading offset: the next 64 channels
-      // (tensor memory begins at 0, all of it being this CTA's, and stages and tiles are unrolled: addresses are constants)
-      auto scores = [&](auto t_, auto stage_) {
-        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
-          mma_f16_ss(t * kN, q_lo + t * (L::kOperand >> 4) + off, k_lo + stage * (L::kOperand >> 4) + off, HI, idesc_s, kk > 0);
-        }
-        tc_commit(bars + Bar::s_full + 8 * t);
-      };
       const int count0 = R.count[0], count1 = R.count[1];
-      if (tmem != 0) fail = 68;
-      if (fail == 0 && count0 > 0) fail = wait_bar<62>(bars + Bar::q_full, 0);
-      if (fail == 0 && count1 > 0) fail = wait_bar<62>(bars + Bar::q_full + 8, 0);
-      if (fail == 0 && steps > 0) {
-        fail = wait_bar<63>(bars + Bar::k_full, 0);
-        if (fail == 0) {
-          tc_fence_after();
-          if (elect_one()) {
-            if (count0 > 0) scores(Int<0>{}, Int<0>{});
-            if (count1 > 0) scores(Int<1>{}, Int<0>{});
-            tc_commit(bars + Bar::k_empty);
-          }
-          __syncwarp();
-        }
-      }
-      auto values = [&](auto t_, auto stage_, auto half_, int j) {                        // 64 keys' part of P V
-        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value, half = decltype(half_)::value;
+      int taken = 0;                       // score tiles issued
+      // S of row tile t and key tile j, as soon as the scores that were in its place have been copied; K's stage is free behind the last
+      auto scores = [&](int t, int j) {
+        if (fail != 0) return;
+        const int before = kSBufs == 1 ? taken : j, buf = kSBufs == 1 ? 0 : t;
+        if (before > 0 && (fail = wait_bar<70>(bars + Bar::s_free + 8 * buf, (before - 1) & 1)) != 0) return;
+        if ((fail = wait_bar<63>(bars + Bar::k_full + 8 * (j & 1), (j >> 1) & 1)) != 0) return;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t a_lo = q_lo + t * (L::kOperand >> 4), b_lo = k_lo + (j & 1) * (L::kOperand >> 4);
 #pragma unroll
-        for (int kk = half * (kN / 32); kk < (half + 1) * (kN / 32); ++kk)
-          mma_f16_ts(256 + t * 128, t * kN + kk * 8, v_lo + stage * (L::kOperand >> 4) + kk * (2048 >> 4), HI, idesc_o, kk > 0 ? 1u : j > 0);
-        tc_commit(bars + (half ? Bar::pv_done : Bar::pv_half) + 8 * t);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * L::kHalf + (kk & 3) * 32) >> 4;
+            mma_f16_ss(kTmS + buf * kN, a_lo + off, b_lo + off, HI, idesc_s, kk > 0);
+          }
+          tc_commit(bars + Bar::s_full + 8 * t);
+          if (t == 1 || j >= count1) tc_commit(bars + Bar::k_empty + 8 * (j & 1));
+        }
+        __syncwarp();
+        ++taken;
       };
-      // Looks at barriers are slow beside busy warps (150 cycles and more), and this warp is held up by the MMAs that it issues, so what a
-      // step needs of keys and values is looked at while the step before waits for weights; only if it is not there yet, again later.
-      bool have_v = false, have_k = false;                     // of the next step
-      auto look = [&](int j) {
-        if (j < steps && !have_v) have_v = __all_sync(0xffffffffu, mbar_test(bars + Bar::v_full + 8 * (j & 1), (j >> 1) & 1));
-        if (j + 1 < steps && !have_k) have_k = __all_sync(0xffffffffu, mbar_test(bars + Bar::k_full + 8 * ((j + 1) & 1), ((j + 1) >> 1) & 1));
-      };
-      auto tile = [&](auto t_, auto stage_, int j, int count) {
-        constexpr int t = decltype(t_)::value, stage = decltype(stage_)::value, next = stage ^ 1;
-        if (fail != 0 || j >= count) return;
+      auto values = [&](int t, int j) {
+        if (fail != 0) return;
+        if ((fail = wait_bar<64>(bars + Bar::v_full + 8 * (j & 1), (j >> 1) & 1)) != 0) return;
         if ((fail = wait_bar<65>(bars + Bar::p_full + 8 * t, j & 1)) != 0) return;
         tc_fence_after();
-        if (elect_one()) values(t_, stage_, Int<0>{}, j);
-        __syncwarp();
-        if (t == 1 || count1 == 0) look(j + 1);
-        if ((fail = wait_bar<65>(bars + Bar::p_full + 16 + 8 * t, j & 1)) != 0) return;
-        tc_fence_after();
         if (elect_one()) {
-          values(t_, stage_, Int<1>{}, j);
-          if (j + 1 < count) scores(t_, Int<next>{});
+          const uint32_t b_lo = v_lo + (j & 1) * (L::kOperand >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kN / 16; ++kk)
+            mma_f16_ts(t * D, kTmP + t * 64 + kk * 8, b_lo + kk * (2048 >> 4), HI, idesc_o, kk > 0 ? 1u : j > 0);
+          tc_commit(bars + Bar::pv_done + 8 * t);
+          if (t == 1 || j >= count1) tc_commit(bars + Bar::v_empty + 8 * (j & 1));
         }
         __syncwarp();
       };
-      auto step = [&](auto stage_, int j) {
-        constexpr int stage = decltype(stage_)::value, next = stage ^ 1;
-        if (!have_v) fail = wait_bar<64>(bars + Bar::v_full + 8 * stage, (j >> 1) & 1);
-        if (fail == 0 && !have_k && j + 1 < steps) fail = wait_bar<63>(bars + Bar::k_full + 8 * next, ((j + 1) >> 1) & 1);
-        have_v = have_k = false;
-        tile(Int<0>{}, stage_, j, count0);
-        tile(Int<1>{}, stage_, j, count1);
-        if (fail != 0) return;
-        if (elect_one()) {
-          tc_commit(bars + Bar::v_empty + 8 * stage);
-          if (j + 1 < steps) tc_commit(bars + Bar::k_empty + 8 * next);
-        }
-        __syncwarp();
-      };
+      if (tmem != 0) fail = 68;            // (all of it is this CTA's)
+      if (fail == 0 && count0 > 0) fail = wait_bar<62>(bars + Bar::q_full, 0);
+      if (fail == 0 && count1 > 0) fail = wait_bar<62>(bars + Bar::q_full + 8, 0);
+      // tiles in turn, each one's next scores in front of its P V, so that they are there when its softmax comes for them
+      if (count0 > 0) scores(0, 0);
+      if (count1 > 0) scores(1, 0);
 #pragma unroll 1
-      for (int j = 0; j < steps && fail == 0; j += 2) {
-        step(Int<0>{}, j);
-        if (j + 1 < steps && fail == 0) step(Int<1>{}, j + 1);
+      for (int j = 0; j < steps && fail == 0; ++j) {
+        if (j + 1 < count0) scores(0, j + 1);
+        if (j < count0) values(0, j);
+        if (j + 1 < count1) scores(1, j + 1);
+        if (j < count1) values(1, j);
       }
       if (fail != 0) {
         give_up(abort_s, P.status, fail);
@@ -272,7 +248,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
         mbar_wait<true>(bars + Bar::drain, 0, 1u << 16);
       }
     }
-    else if (warp == 17) {
+    else if (warp == 13) {
       // ---------------------------------------------------------------- records, by bulk copies; which there are goes along
       volatile uint32_t* const there_s = reinterpret_cast<volatile uint32_t*>(smem + L::bars + Bar::there);
       const int64_t page_bytes = (int64_t)A.Hkv * (A.page_size / 16) * Rec::kBytes;
@@ -307,99 +283,101 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- cache -> fp16 tiles: a warp 32 keys of each
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFillRegs));
-    const bool keys = warp < 12;
     const int w = warp & 3, n = lane >> 2, c = lane & 3;
-    const uint32_t raw_at = base + L::raw + 2 * w * Rec::kBytes, codes_from = raw_at + (keys ? 0 : Rec::kValues);
+    const uint32_t raw_at = base + L::raw + 2 * w * Rec::kBytes;
     const volatile uint32_t* const there_s = reinterpret_cast<const volatile uint32_t*>(smem + L::bars + Bar::there);
     constexpr int W = D / 32;                                  // words of a lane's codes of a token (keys), of two tokens (values)
     // D=128: half of the lanes take the halves of their 16 bytes in the other order, so that 8 lanes' stores meet different banks.  Keys:
     // rows n, n + 1 and channels 32 c ... fall on the same 128 bytes for c and c + 2.  Values: blocks n and n + 1 do.
-    const bool turn = D == 128 && (keys ? c >= 2 : n & 1);
-    const uint32_t codes_at = codes_from + lane * 4 * W, first = turn ? 8 : 0, second = turn ? 0 : 8;
+    const bool turn_k = D == 128 && c >= 2, turn_v = D == 128 && (n & 1);
     const uint32_t scales_at = raw_at + Rec::kValueScales + (D == 128 ? lane * 4 : (lane >> 3) * 16 + c * 4);
+    auto codes = [&](uint32_t at, bool turn, uint32_t (&x)[W]) {
+      if constexpr (D == 128) {
+        const uint2 u = lds64(at + lane * 16 + (turn ? 8 : 0)), v = lds64(at + lane * 16 + (turn ? 0 : 8));
+        x[0] = u.x; x[1] = u.y; x[2] = v.x; x[3] = v.y;
+      } else {
+        const uint2 u = lds64(at + lane * 8);
+        x[0] = u.x; x[1] = u.y;
+      }
+    };
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
       const int stage = j & 1, key0 = key_begin + j * kN + w * 32;
       // two records to registers, so that the next can come
       if ((fail = wait_bar<69>(bars + Bar::raw_full, j & 1)) != 0) break;
       const uint32_t there = *there_s >> (2 * w);
-      uint32_t x[2][2][W], ks[2] = {0, 0}, vsc[2];
+      uint32_t kx[2][2][W], vx[2][2][W], ks[2], vsc[2], poison[2] = {0, 0};
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
+        const uint32_t rec = raw_at + r * Rec::kBytes;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t at = codes_at + r * Rec::kBytes + i * 4 * D;
-          if constexpr (D == 128) {
-            const uint2 u = lds64(at + first), v = lds64(at + second);
-            x[r][i][0] = u.x; x[r][i][1] = u.y; x[r][i][2] = v.x; x[r][i][3] = v.y;
-          } else {
-            const uint2 u = lds64(at);
-            x[r][i][0] = u.x; x[r][i][1] = u.y;
-          }
+          codes(rec + i * 4 * D, turn_k, kx[r][i]);
+          codes(rec + Rec::kValues + i * 4 * D, turn_v, vx[r][i]);
         }
         vsc[r] = lds32(scales_at + r * Rec::kBytes);
-        if (keys) ks[r] = D == 128 ? lds32(raw_at + r * Rec::kBytes + Rec::kKeyScales + lane * 4) : lds16(raw_at + r * Rec::kBytes + Rec::kKeyScales + lane * 2);
+        ks[r] = D == 128 ? lds32(rec + Rec::kKeyScales + lane * 4) : lds16(rec + Rec::kKeyScales + lane * 2);
         if (!(there >> r & 1)) ks[r] = vsc[r] = 0;             // (zeros, then; a page there is not masks its keys as well)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + Bar::raw_empty);
-      if (j >= 2) {
-        fail = keys ? wait_bar<60>(bars + Bar::k_empty + 8 * stage, ((j >> 1) - 1) & 1) : wait_bar<61>(bars + Bar::v_empty + 8 * stage, ((j >> 1) - 1) & 1);
-        if (fail != 0) break;
-      }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        uint32_t poison = 0;
+      for (int r = 0; r < 2; ++r)
         if (key0 + 16 * r + 16 > see_any || __any_sync(0xffffffffu, (((vsc[r] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0)) {
           const uint2 u = mend_scales(vsc[r], see_any - key0 - 16 * r);
-          vsc[r] = u.x; poison = u.y;
+          vsc[r] = u.x; poison[r] = u.y;
         }
-        if (keys) {
-          const uint32_t sk = base + L::k + stage * L::kOperand;
-          const uint32_t f0 = e4m3x2_to_f16(ks[r]), f1 = D == 128 ? e4m3x2_to_f16(ks[r] >> 16) : f0;
+      if (j >= 2 && (fail = wait_bar<60>(bars + Bar::k_empty + 8 * stage, ((j >> 1) - 1) & 1)) != 0) break;
+      const uint32_t sk = base + L::k + stage * L::kOperand, sv = base + L::v + stage * L::kOperand;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {                        // tokens n, n + 8
-            const int row = w * 32 + r * 16 + i * 8 + n;
-            uint32_t sc[2];
-            if constexpr (D == 128) {
-              sc[0] = __byte_perm(i ? f1 : f0, 0, turn ? 0x3232 : 0x1010); sc[1] = __byte_perm(i ? f1 : f0, 0, turn ? 0x1010 : 0x3232);
-            } else {
-              sc[0] = sc[1] = __byte_perm(f0, 0, i ? 0x3232 : 0x1010);
-            }
-            if (poison >> i & 1) sc[0] = sc[1] = 0x7e007e00u;
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t f0 = e4m3x2_to_f16(ks[r]), f1 = D == 128 ? e4m3x2_to_f16(ks[r] >> 16) : f0;
 #pragma unroll
-            for (int z = 0; z < W; ++z) {
-              uint32_t y[4];
-              e2m1x8_to_f16(x[r][i][z], y);
-#pragma unroll
-              for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc[D == 128 ? z >> 1 : 0]);
-              sts128(sk + L::at(row, c * W + (turn ? z ^ 2 : z)), y);
-            }
+        for (int i = 0; i < 2; ++i) {                          // tokens n, n + 8
+          const int row = w * 32 + r * 16 + i * 8 + n;
+          uint32_t sc[2];
+          if constexpr (D == 128) {
+            sc[0] = __byte_perm(i ? f1 : f0, 0, turn_k ? 0x3232 : 0x1010); sc[1] = __byte_perm(i ? f1 : f0, 0, turn_k ? 0x1010 : 0x3232);
+          } else {
+            sc[0] = sc[1] = __byte_perm(f0, 0, i ? 0x3232 : 0x1010);
           }
-        } else {
-          const uint32_t sv = base + L::v + stage * L::kOperand;
+          if (poison[r] >> i & 1) sc[0] = sc[1] = 0x7e007e00u;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {                        // tokens 2 c + 8 i and the next, or (turn) the other way round
-            const uint32_t f = e4m3x2_to_f16(vsc[r] >> (16 * i));
+          for (int z = 0; z < W; ++z) {
+            uint32_t y[4];
+            e2m1x8_to_f16(kx[r][i][z], y);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int row = w * 32 + r * 16 + i * 8 + 2 * c + (turn ? e ^ 1 : e);
-              const uint32_t sc = __byte_perm(f, 0, (turn ? e == 0 : e == 1) ? 0x3232 : 0x1010);
-#pragma unroll
-              for (int z = 0; z < W / 2; ++z) {
-                uint32_t y[4];
-                e2m1x8_to_f16(x[r][i][e * (W / 2) + z], y);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc);
-                sts128(sv + L::at(row, n * (W / 2) + z), y);
-              }
-            }
+            for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc[D == 128 ? z >> 1 : 0]);
+            sts128(sk + L::at(row, c * W + (turn_k ? z ^ 2 : z)), y);
           }
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars + (keys ? Bar::k_full : Bar::v_full) + 8 * stage);
+      if (lane == 0) mbar_arrive(bars + Bar::k_full + 8 * stage);
+      if (j >= 2 && (fail = wait_bar<61>(bars + Bar::v_empty + 8 * stage, ((j >> 1) - 1) & 1)) != 0) break;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                          // tokens 2 c + 8 i and the next, or (turn) the other way round
+          const uint32_t f = e4m3x2_to_f16(vsc[r] >> (16 * i));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = w * 32 + r * 16 + i * 8 + 2 * c + (turn_v ? e ^ 1 : e);
+            const uint32_t sc = __byte_perm(f, 0, (turn_v ? e == 0 : e == 1) ? 0x3232 : 0x1010);
+#pragma unroll
+            for (int z = 0; z < W / 2; ++z) {
+              uint32_t y[4];
+              e2m1x8_to_f16(vx[r][i][e * (W / 2) + z], y);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) y[u] = hmul2(y[u], sc);
+              sts128(sv + L::at(row, n * (W / 2) + z), y);
+            }
+          }
+        }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + Bar::v_full + 8 * stage);
     }
     if (fail != 0) give_up(abort_s, P.status, fail);
   } else {
@@ -409,7 +387,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
     const bool real = row < rows;
     const int tok = real ? row / P.group : 0, hq = h * P.group + (real ? row - tok * P.group : 0);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tm_s = tmem + t * kN + lanes, tm_o = tmem + 256 + t * 128 + lanes;
+    const uint32_t tm_s = tmem + kTmS + (kSBufs == 1 ? 0 : t) * kN + lanes, tm_o = tmem + t * D + lanes, tm_p = tmem + kTmP + t * 64 + lanes;
     float factor, add = 0.f;
     {
       const uint4* const src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)A.q + (int64_t)(seq.q0 + tok) * A.q_sn + hq * A.q_sh);
@@ -453,98 +431,84 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
     const int limit_all = __reduce_min_sync(0xffffffffu, limit);
     float m = kLowest;
     float2 l = make_float2(0.f, 0.f);
-    // One key tile.  Scores come by 32 columns, the next ones on their way while these are worked on.  Masks and what else is rare stay out
-    // of the loop that nearly all tiles take: as one loop with branches it took a third longer, its code being fetched rather
-    // than run.
+    // One key tile: its scores to registers, so that the next ones can be on their way, then their weights.  Masks stay out of the loop that
+    // nearly all tiles take.
     auto key_tile = [&](auto masked_, int j) {
       constexpr bool masked = decltype(masked_)::value != 0;
       if ((fail = wait_bar<66>(bars + Bar::s_full + 8 * t, j & 1)) != 0) return;
       tc_fence_after();
-      const int key0 = key_begin + j * kN;
-      auto mask = [&](int i, uint32_t (&s)[32]) {              // 32 scores from key 32 i of the tile on
-        const int key = key0 + 32 * i;
+      uint32_t s[4][32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x)
-          if (key + x >= limit) s[x] = 0xff800000u;
+      for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, s[i]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + Bar::s_free + 8 * (kSBufs == 1 ? 0 : t));
+      if (masked) {
+        const int key0 = key_begin + j * kN;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (key0 + 32 * i + x >= limit) s[i][x] = 0xff800000u;
         if (absent) {                      // some page of the item's keys is not in the cache (the whole CTA knows)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-            if (key + 16 * y < key_end && !has_page(key + 16 * y)) {
+          for (int i = 0; i < 8; ++i)
+            if (key0 + 16 * i < key_end && !has_page(key0 + 16 * i)) {
 #pragma unroll
-              for (int x = 0; x < 16; ++x) s[16 * y + x] = 0xff800000u;
+              for (int x = 0; x < 16; ++x) s[i >> 1][(i & 1) * 16 + x] = 0xff800000u;
             }
         }
-      };
-      uint32_t s0[32], s1[32];
-      tmem_ld32(tm_s, s0);
+      }
+      if (j > 0 && (fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (j - 1) & 1)) != 0) return;         // P's place is free
+      tc_fence_after();
+      float2 both;
+#pragma unroll 1
+      for (bool again = false;; again = true) {
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float2 f2 = make_float2(factor, factor), base2 = make_float2(kTop - m, kTop - m);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[2][16];
-        float2 sum[2];
-        auto weights = [&](const uint32_t (&s)[32], uint32_t (&w)[16]) {
-          const float2 f2 = make_float2(factor, factor), base2 = make_float2(kTop - m, kTop - m);
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[16];
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
-            float2 e = ffma2(make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), f2, base2);
+            float2 e = ffma2(make_float2(__uint_as_float(s[i][2 * x]), __uint_as_float(s[i][2 * x + 1])), f2, base2);
             e.x = ex2_approx(e.x); e.y = ex2_approx(e.y);
             sum[x & 1] = fadd2(sum[x & 1], e);
-            w[x] = pack_f16(e.x, e.y);
+            p[x] = pack_f16(e.x, e.y);
           }
-        };
-        float2 both;
-#pragma unroll 1
-        for (bool again = false;; again = true) {
-          sum[0] = sum[1] = make_float2(0.f, 0.f);
-          tmem_wait_ld_of(s0);
-          tmem_ld32(tm_s + 64 * half + 32, s1);
-          if (masked) mask(2 * half, s0);
-          weights(s0, p[0]);
-          tmem_wait_ld_of(s1);
-          if (masked) mask(2 * half + 1, s1);
-          weights(s1, p[1]);
-          both = fadd2(sum[0], sum[1]);
-          // a weight too large for fp16 makes the sum larger than 2^15 (and where it is, one of the 64 is 2^9 at least); so does a NaN
-          const bool bad = !(both.x + both.y <= 32768.f) || m == kLowest;
-          if (__builtin_expect(again || !__any_sync(0xffffffffu, bad), 1)) break;
-          // once more with the maximum of these 64 scores.  Rows that are well get the same weights again: no row's bits depend on
-          // another row.
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int i = 0; i < 2; ++i) {
-            tmem_ld32(tm_s + 64 * half + 32 * i, s1);
-            tmem_wait_ld_of(s1);
-            if (masked) mask(2 * half + i, s1);
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) top = fmaxf(top, fmaxf(__uint_as_float(s1[x]), __uint_as_float(s1[x + 1])));
-          }
-          const float m_new = bad ? fmaxf(m, top * factor) : m, corr = ex2_approx(m - m_new);
-          m = m_new;
-          l.x *= corr; l.y *= corr;
-          if (j > 0 || half == 1) {
-            fail = half == 0 ? wait_bar<67>(bars + Bar::pv_done + 8 * t, (j - 1) & 1) : wait_bar<67>(bars + Bar::pv_half + 8 * t, j & 1);
-            if (fail != 0) return;
-            tc_fence_after();
-#pragma unroll 1
-            for (int i = 0; i < D / 16; ++i) {
-              uint32_t o[16];
-              tmem_ld16(tm_o + 16 * i, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
-              tmem_st16(tm_o + 16 * i, o);
-            }
-          }
-          tmem_ld32(tm_s + 64 * half, s0);
+          tmem_st16(tm_p + 16 * i, p);
         }
-        l = fadd2(l, both);
-        tmem_st16(tm_s + 32 * half, p[0]);
-        tmem_st16(tm_s + 32 * half + 16, p[1]);
-        if (half == 0) tmem_ld32(tm_s + 64, s0);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + Bar::p_full + 16 * half + 8 * t);
+        both = fadd2(sum[0], sum[1]);
+        // a weight too large for fp16 makes the sum larger than 2^15 (and where it is, one of the 128 is 2^8 at least); so does a NaN
+        const bool bad = !(both.x + both.y <= 32768.f) || m == kLowest;
+        if (__builtin_expect(again || !__any_sync(0xffffffffu, bad), 1)) break;
+        // Once more with the maximum of these scores.  Rows that are well get the same weights again: no row's bits depend on another row.
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) top = fmaxf(top, fmaxf(__uint_as_float(s[i][x]), __uint_as_float(s[i][x + 1])));
+        const float m_new = bad ? fmaxf(m, top * factor) : m, corr = ex2_approx(m - m_new);
+        m = m_new;
+        l.x *= corr; l.y *= corr;
+        if (j > 0) {
+#pragma unroll 1
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t o[16];
+            tmem_ld16(tm_o + 16 * i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+            tmem_st16(tm_o + 16 * i, o);
+          }
+        }
       }
+      l = fadd2(l, both);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + Bar::p_full + 8 * t);
     };
     const int plain = absent ? 0 : max(0, min(count, (limit_all - key_begin) / kN));     // tiles all of whose keys every row of the warp sees
     int j = 0;
@@ -598,7 +562,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
