@@ -437,6 +437,8 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
       constexpr bool masked = decltype(masked_)::value != 0;
       if ((fail = wait_bar<66>(bars + Bar::s_full + 8 * t, j & 1)) != 0) return;
       tc_fence_after();
+      // (whether P's place is free: a look takes hundreds of cycles beside busy warps, so it lies beside the copy)
+      const bool place_free = j == 0 || mbar_test(bars + Bar::pv_done + 8 * t, (j - 1) & 1);
       uint32_t s[4][32];
 #pragma unroll
       for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, s[i]);
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
             }
         }
       }
-      if (j > 0 && (fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (j - 1) & 1)) != 0) return;         // P's place is free
+      if (!__all_sync(0xffffffffu, place_free) && (fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (j - 1) & 1)) != 0) return;
       tc_fence_after();
       float2 both;
 #pragma unroll 1
