@@ -5,12 +5,15 @@
 // Scores are taken transposed, S^T = K Q^T: the keys are the A operand of mma.sync (m16n8k16, fp16 in, fp32 out), 16 of them per
 // instruction, and 8 query rows the B operand; O^T = V^T P^T likewise.  With queries as A 16 rows would be paid for 8.  An E2M1 value times
 // its E4M3 scale has 6 significant bits and lies between 2^-10 and 2688, exact in fp16; queries are scaled by a power of two per
-// row, so that their 8 bits are exact too (down to 2^-31 of the row's largest).  P is rounded to fp16 once (2^-12 relative), with its
-// maximum put at 2^8 so that small ones keep their bits down to 2^-22 of it; sums are fp32.
+// row, so that their 8 bits are exact too (down to 2^-31 of the row's largest).  P is rounded to fp16 once (by 2^-11 at most), with its
+// maximum put at 2^6 so that small ones keep their bits down to 2^-20 of it; sums are fp32.
 //
 // A CTA has four warps; each fetches chunks of 32 keys by cp.async into a ring of its own, so nothing in the loop waits for another warp.
-// The four, and then parts of a row that several CTAs have (a second small kernel, launched as a programmatic dependent), are joined
-// by their maxima and sums in a fixed order.
+// The four, and then parts of a row that several CTAs have (through a cluster's shared memory, or by a second small kernel, launched as a
+// programmatic dependent), are joined by their maxima and sums in a fixed order.
+//
+// What bounds it: a key costs D 9/8 bytes and, whatever the rows, the instructions that turn its codes into fp16.  32 sequences of 8192 keys, 32
+// heads of 8, D=128: 62 us, 4.9 TB/s; the chip's copy does 6.5.  Short caches are bound by latency: 1000 keys of one sequence 5.2 us.
 #include "kernels.h"
 #include "kv_attn.cuh"
 
@@ -18,7 +21,7 @@ namespace sage3 {
 
 namespace {
 
-constexpr int kWarps = 4, kChunk = 32, kStages = 3, kBlock = kWarps * kChunk;
+constexpr int kWarps = 4, kChunk = 32, kStages = 3, kBlock = kWarps * kChunk, kMostParts = 8;
 
 struct Header {                           // at the front of the workspace, for the joining kernel
   int per;                                // units of work per CTA
@@ -27,6 +30,7 @@ struct Header {                           // at the front of the workspace, for 
 struct Params {
   KvAttnArgs a;
   int group, tiles, page_shift;           // query heads per kv head; tiles of rows of the longest sequence
+  int parts;                              // CTAs of a cluster
   uint32_t group_inverse;                 // 2^32 / group rounded up: exact for quotients of the few rows there are
   float scale_log2;
   Header* header;
@@ -59,10 +63,26 @@ __device__ __forceinline__ int blocks_of(const KvSeq& s) { return max(1, (s.kv_l
 template <int kRows>
 __device__ __forceinline__ int tiles_of(const KvSeq& s, int group) { return (s.q_len * group + kRows - 1) / kRows; }
 
+// shared memory: the rings, and in their place at the end the four warps' results and (clusters) the CTA's own
 template <int D, int NB>
-constexpr int smem_bytes() {
-  return kWarps * kStages * (kChunk / 16) * 18 * D > kWarps * 8 * NB * ((D + 4) * 4 + 8) ? kWarps * kStages * (kChunk / 16) * 18 * D
-                                                                                        : kWarps * 8 * NB * ((D + 4) * 4 + 8);
+struct Smem {
+  static constexpr int kRows = 8 * NB, kRing = kWarps * kStages * (kChunk / 16) * 18 * D;
+  static constexpr int o = 0, ml = kWarps * kRows * (D + 4) * 4, part = ml + kWarps * kRows * 8, part_ml = part + kRows * D * 4, end = part_ml + kRows * 8;
+  static constexpr int bytes = kRing > end ? kRing : end;
+};
+
+__device__ __forceinline__ uint32_t of_cta(uint32_t at, int rank) {                     // the same place in the cluster's CTA `rank`
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 ld_cluster(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // CTAs per SM that the registers are held to
@@ -71,9 +91,12 @@ constexpr int ctas_per_sm(int D, int NB) { return NB == 1 ? 4 : NB == 2 ? 3 : D 
 // The work: an item is a (sequence, kv head, tile of rows), a unit one of its blocks of 128 keys.  All units, in this order, are dealt out in
 // equal runs, so that ragged batches and single long sequences fill the chip alike; a CTA's run may end inside an item and go on to
 // others.  Only its first and its last item can be shared with other CTAs: two places for partial results each.
-template <int D, int NB>                  // stored head dim, 8-row blocks
+// kCluster, for little work: a cluster of CTAs has an item, and its parts are joined through their shared memory; there is nothing to
+// look up in front and no second kernel.
+template <int D, int NB, bool kCluster>   // stored head dim, 8-row blocks
 __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_kernel(const Params P) {
   using Rec = KvRecord<D>;
+  using L = Smem<D, NB>;
   constexpr int kRows = 8 * NB, kRecs = kChunk / 16, kStageBytes = kRecs * Rec::kBytes;
   constexpr int kKS = D / 16;             // k steps of the scores = tiles of 16 channels of the output
   extern __shared__ __align__(16) uint8_t sm[];
@@ -81,63 +104,18 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
   __shared__ float add_s[kRows];
   const KvAttnArgs& A = P.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
-  pdl_launch_dependents();
+  if (!kCluster) pdl_launch_dependents();
 
   auto group_of = [&](int row) { return P.group == 1 ? row : (int)__umulhi((uint32_t)row, P.group_inverse); };       // row / group
 
-  // ---- this CTA's units
-  auto units = [&](int b) {
-    const KvSeq s(A, b);
-    return A.Hkv * tiles_of<kRows>(s, P.group) * blocks_of(s);
-  };
-  // a thread has some sequences next to one another; one scan gives it the units in front of them, and their total
-  const int each = (A.B + kWarps * 32 - 1) / (kWarps * 32), b_first = min((int)threadIdx.x * each, A.B), b_last = min(b_first + each, A.B);
-  int mine = 0;
-  for (int b = b_first; b < b_last; ++b) mine += units(b);
-  int incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += x;
-  }
-  if (lane == 31) scan_s[warp] = incl;
-  __syncthreads();
-  int total = 0, before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += scan_s[w];
-    total += scan_s[w];
-  }
-  const int per = (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x);
-  int unit = blockIdx.x * per;
-  const int unit_end = min(unit + per, total);
-  if (blockIdx.x == 0 && threadIdx.x == 0) P.header->per = per;
-  if (unit >= unit_end) return;
-  if (unit >= before && unit < before + mine) {                // one of this thread's is the first
-    int b = b_first, x = before;
-    for (int n_b; unit >= x + (n_b = units(b)); ++b) x += n_b;
-    where_s[0] = b; where_s[1] = x;
-  }
-  __syncthreads();
-  int b = where_s[0];
-  int rest = unit - where_s[1];            // units of sequence b before this one
-
-#pragma unroll 1
-  while (unit < unit_end) {
-    const KvSeq seq(A, b);
-    const int blocks = blocks_of(seq), tiles = tiles_of<kRows>(seq, P.group);
-    if (rest >= A.Hkv * tiles * blocks) {             // on to the next sequence
-      rest -= A.Hkv * tiles * blocks;
-      if (++b >= A.B) break;
-      continue;
-    }
-    const int item = rest / blocks, block = rest - item * blocks, take = min(blocks - block, unit_end - unit);
-    const int h = item / tiles, tile = item - h * tiles, bh = b * A.Hkv + h;
+  // ---- a part of an item: `take` blocks from `block` on
+  auto item_part = [&](const KvSeq& seq, int b, int h, int tile, int block, int take, int blocks) {
+    const int bh = b * A.Hkv + h;
     const int rows = seq.q_len * P.group, row0 = tile * kRows;
     const int last_row = min(rows, row0 + kRows) - 1;
     const int see_all = seq.seen(A, group_of(row0)), see_any = seq.seen(A, group_of(last_row));   // keys that each row, that any row sees
     const int begin = block * kBlock, end = min(begin + take * kBlock, see_any);
-    const bool whole = take == blocks, head_of_item = block == 0;
+    [[maybe_unused]] const bool whole = take == blocks, head_of_item = block == 0 || kCluster;
 
     // ---- queries under way: this lane the channels c D/4 ... of row n of each block (used when keys have been asked for: both take as long)
     uint4 q_raw[NB][D / 32];
@@ -426,8 +404,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
 
     // ---- join the four warps
     __syncthreads();
-    float* const o_s = reinterpret_cast<float*>(sm);                      // [warp][row][D + 4]
-    float2* const ml_s = reinterpret_cast<float2*>(sm + kWarps * kRows * (D + 4) * 4);
+    float* const o_s = reinterpret_cast<float*>(sm + L::o);               // [warp][row][D + 4]
+    float2* const ml_s = reinterpret_cast<float2*>(sm + L::ml);
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
 #pragma unroll
@@ -466,26 +444,129 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
           const float2 x = *reinterpret_cast<const float2*>(o_s + (w * kRows + row) * (D + 4) + lane * kPer + k);
           acc[k] = fmaf(wgt[w], x.x, acc[k]); acc[k + 1] = fmaf(wgt[w], x.y, acc[k + 1]);
         }
-      const int tok = group_of(row0 + row), hq = h * P.group + row0 + row - tok * P.group;
-      if (whole) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh + lane * kPer;
-        if (lane * kPer < A.D)
+      if constexpr (kCluster) {
 #pragma unroll
-          for (int k = 0; k < kPer; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pack_bf16(acc[k] * inv, acc[k + 1] * inv);
-        if (lane == 0 && A.lse != nullptr) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, add_s[row]);
+        for (int k = 0; k < kPer; k += 2) reinterpret_cast<float2*>(sm + L::part)[(row * D + lane * kPer + k) / 2] = make_float2(acc[k], acc[k + 1]);
+        if (lane == 0) reinterpret_cast<float2*>(sm + L::part_ml)[row] = make_float2(m, l);
       } else {
-        const int64_t at = ((int64_t)blockIdx.x * 2 + (head_of_item ? 1 : 0)) * kRows + row;
+        const int tok = group_of(row0 + row), hq = h * P.group + row0 + row - tok * P.group;
+        if (whole) {
+          const float inv = l == 0.f ? 0.f : 1.0f / l;
+          __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh + lane * kPer;
+          if (lane * kPer < A.D)
 #pragma unroll
-        for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(P.o_part + at * D + lane * kPer + k) = make_float2(acc[k], acc[k + 1]);
-        if (lane == 0) P.ml_part[at] = make_float2(m, l);
-        if (lane == 0 && head_of_item && A.lse != nullptr) P.lse_add[((int64_t)bh * P.tiles + tile) * kRows + row] = add_s[row];
+            for (int k = 0; k < kPer; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pack_bf16(acc[k] * inv, acc[k + 1] * inv);
+          if (lane == 0 && A.lse != nullptr) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, add_s[row]);
+        } else {
+          const int64_t at = ((int64_t)blockIdx.x * 2 + (head_of_item ? 1 : 0)) * kRows + row;
+#pragma unroll
+          for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(P.o_part + at * D + lane * kPer + k) = make_float2(acc[k], acc[k + 1]);
+          if (lane == 0) P.ml_part[at] = make_float2(m, l);
+          if (lane == 0 && head_of_item && A.lse != nullptr) P.lse_add[((int64_t)bh * P.tiles + tile) * kRows + row] = add_s[row];
+        }
       }
     }
-    if (head_of_item && threadIdx.x == 0) P.item_start[(int64_t)bh * P.tiles + tile] = unit;
-    unit += take;
-    rest += take;
-    __syncthreads();                       // the ring is the next item's
+  };
+
+  if constexpr (kCluster) {
+    const int item = blockIdx.x / P.parts, part = blockIdx.x - item * P.parts, bh = item / P.tiles, tile = item - bh * P.tiles;
+    const int b = bh / A.Hkv, h = bh - b * A.Hkv;
+    const KvSeq seq(A, b);
+    const int rows = seq.q_len * P.group, row0 = tile * kRows;
+    if (row0 >= rows) return;              // (the whole cluster)
+    const int blocks = blocks_of(seq), per = (blocks + P.parts - 1) / P.parts, block = min(part * per, blocks);
+    item_part(seq, b, h, tile, block, min(per, blocks - block), blocks);
+    cluster_sync();
+    // rows dealt out to the CTAs' warps, parts in the order of the keys
+    constexpr int kPer = D / 32;
+    const uint32_t at_o = smem_u32(sm + L::part), at_ml = smem_u32(sm + L::part_ml);
+#pragma unroll 1
+    for (int row = part + P.parts * warp; row < kRows && row0 + row < rows; row += P.parts * kWarps) {
+      float2 ml = make_float2(kLowest, 0.f);
+      if (lane < P.parts) ml = ld_cluster(of_cta(at_ml + row * 8, lane));
+      float m = ml.x;
+#pragma unroll
+      for (int d = 4; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      m = __shfl_sync(0xffffffffu, m, 0);
+      const float mine = ex2_approx(ml.x - m);
+      float acc[kPer], l = 0.f;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
+#pragma unroll
+      for (int x = 0; x < kMostParts; ++x) {
+        const float w = __shfl_sync(0xffffffffu, mine, x), lx = __shfl_sync(0xffffffffu, ml.y, x);
+        if (x < P.parts) {
+          l = fmaf(w, lx, l);
+#pragma unroll
+          for (int k = 0; k < kPer; k += 2) {
+            const float2 v = ld_cluster(of_cta(at_o + (row * D + lane * kPer + k) * 4, x));
+            acc[k] = fmaf(w, v.x, acc[k]); acc[k + 1] = fmaf(w, v.y, acc[k + 1]);
+          }
+        }
+      }
+      const int tok = group_of(row0 + row), hq = h * P.group + row0 + row - tok * P.group;
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh + lane * kPer;
+      if (lane * kPer < A.D)
+#pragma unroll
+        for (int k = 0; k < kPer; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pack_bf16(acc[k] * inv, acc[k + 1] * inv);
+      if (lane == 0 && A.lse != nullptr) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, add_s[row]);
+    }
+    cluster_sync();                        // nobody's shared memory goes while another reads it
+  } else {
+    // ---- this CTA's units
+    auto units = [&](int b) {
+      const KvSeq s(A, b);
+      return A.Hkv * tiles_of<kRows>(s, P.group) * blocks_of(s);
+    };
+    // a thread has some sequences next to one another; one scan gives it the units in front of them, and their total
+    const int each = (A.B + kWarps * 32 - 1) / (kWarps * 32), b_first = min((int)threadIdx.x * each, A.B), b_last = min(b_first + each, A.B);
+    int mine = 0;
+    for (int b = b_first; b < b_last; ++b) mine += units(b);
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += x;
+    }
+    if (lane == 31) scan_s[warp] = incl;
+    __syncthreads();
+    int total = 0, before = incl - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan_s[w];
+      total += scan_s[w];
+    }
+    const int per = (int)(((uint32_t)total + gridDim.x - 1) / gridDim.x);
+    int unit = blockIdx.x * per;
+    const int unit_end = min(unit + per, total);
+    if (blockIdx.x == 0 && threadIdx.x == 0) P.header->per = per;
+    if (unit >= unit_end) return;
+    if (unit >= before && unit < before + mine) {                // one of this thread's is the first
+      int b = b_first, x = before;
+      for (int n_b; unit >= x + (n_b = units(b)); ++b) x += n_b;
+      where_s[0] = b; where_s[1] = x;
+    }
+    __syncthreads();
+    int b = where_s[0];
+    int rest = unit - where_s[1];            // units of sequence b before this one
+
+#pragma unroll 1
+    while (unit < unit_end) {
+      const KvSeq seq(A, b);
+      const int blocks = blocks_of(seq), tiles = tiles_of<kRows>(seq, P.group);
+      if (rest >= A.Hkv * tiles * blocks) {             // on to the next sequence
+        rest -= A.Hkv * tiles * blocks;
+        if (++b >= A.B) break;
+        continue;
+      }
+      const int item = rest / blocks, block = rest - item * blocks, take = min(blocks - block, unit_end - unit), h = item / tiles, tile = item - h * tiles;
+      item_part(seq, b, h, tile, block, take, blocks);
+      if (block == 0 && threadIdx.x == 0) P.item_start[(int64_t)(b * A.Hkv + h) * P.tiles + tile] = unit;
+      unit += take;
+      rest += take;
+      __syncthreads();                       // the ring is the next item's
+    }
   }
 }
 
@@ -585,6 +666,7 @@ inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct Plan {
   int nb, tiles;
+  int parts;                              // CTAs of a cluster; 0: equal runs
   int64_t ctas, units, rows;              // units and rows (padded to tiles), counted in 32 bits by the kernels
   size_t starts, adds, ml, o;             // offsets in the workspace
   size_t bytes;
@@ -600,21 +682,39 @@ Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
   const int64_t fit = (int64_t)sms * ctas_per_sm(DS, p.nb);
   p.units = items * blocks;
   p.rows = items * 8 * p.nb;
+  // Clusters where all of them fit at once and none has far to go: up to 4 blocks per CTA, 8 where a third of the chip is had anyway (us, equal
+  // runs -> clusters, D=128: B1, 32 heads of 8, 1000 keys 6.4 -> 5.2, 4096 8.1 -> 7.6, 16384 12.8 -> 16.6; B4 1000 keys 7.7 -> 6.3, 8192
+  // 15.6 -> 13.8; B3 of 6 tokens 4096 keys 20.0 -> 15.8).  Longer ones, and ragged ones of more keys, are better off in equal runs; one
+  // block needs no joining (100 keys 4.1 -> 4.6).
+  p.parts = 2;
+  while (p.parts < blocks && p.parts < kMostParts) p.parts *= 2;
+  if (blocks < 2 || items * p.parts > fit || blocks > (3 * items * p.parts >= fit ? 8 : 4) * p.parts) p.parts = 0;
   p.ctas = p.units < fit ? p.units : fit;
   p.starts = 256;
   p.adds = p.starts + align256(items * 4);
   p.ml = p.adds + align256(items * 8 * p.nb * 4);
   p.o = p.ml + align256(p.ctas * 2 * 8 * p.nb * 8);
-  p.bytes = p.o + align256(p.ctas * 2 * 8 * p.nb * DS * 4);
+  p.bytes = p.parts != 0 ? 256 : p.o + align256(p.ctas * 2 * 8 * p.nb * DS * 4);
   return p;
 }
 
 template <int D, int NB>
 cudaError_t launch(const Params& P, const Plan& p, bool split, cudaStream_t stream) {
-  constexpr int smem = smem_bytes<D, NB>();
+  constexpr int smem = Smem<D, NB>::bytes;
+  if (p.parts != 0) {
+    static std::atomic<uint64_t> allowed;
+    if (cudaError_t e = allow_smem(kv_decode_kernel<D, NB, true>, smem, allowed); e != cudaSuccess) return e;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)(P.a.B * P.a.Hkv * P.tiles * p.parts)); c.blockDim = dim3(kWarps * 32); c.dynamicSmemBytes = smem; c.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = p.parts; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    c.attrs = &at; c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kv_decode_kernel<D, NB, true>, P);
+  }
   static std::atomic<uint64_t> allowed;
-  if (cudaError_t e = allow_smem(kv_decode_kernel<D, NB>, smem, allowed); e != cudaSuccess) return e;
-  if (cudaError_t e = launch_pdl(kv_decode_kernel<D, NB>, dim3((unsigned)p.ctas), kWarps * 32, smem, stream, false, P); e != cudaSuccess) return e;
+  if (cudaError_t e = allow_smem(kv_decode_kernel<D, NB, false>, smem, allowed); e != cudaSuccess) return e;
+  if (cudaError_t e = launch_pdl(kv_decode_kernel<D, NB, false>, dim3((unsigned)p.ctas), kWarps * 32, smem, stream, false, P); e != cudaSuccess) return e;
   if (!split) return cudaGetLastError();
   const int64_t items = (int64_t)P.a.B * P.a.Hkv * P.tiles, rows = items * 8 * NB;
   if (items * 8 <= p.ctas) return launch_pdl(kv_join_kernel<D, NB, true>, dim3((unsigned)rows), 128, 0, stream, true, P);
@@ -640,6 +740,7 @@ cudaError_t launch_kv_decode(const KvAttnArgs& a, cudaStream_t stream) {
   P.group = a.Hq / a.Hkv; P.tiles = p.tiles;
   P.group_inverse = (uint32_t)(0xffffffffu / (uint32_t)P.group) + 1;
   P.scale_log2 = a.sm_scale * kLog2e;
+  P.parts = p.parts;
   P.page_shift = 0;
   while ((1 << P.page_shift) < a.page_size) ++P.page_shift;
   char* const w = (char*)a.workspace;

@@ -86,7 +86,8 @@ def attend(q, data, D, page_size, table, kv_lens, q_lens, causal=True, scale=Non
 
     The bounds.  Codes times scales and queries are exact in the kernels.  A score is a sum of D products in fp32, each addition of which
     may lose a unit in the last place of the largest partial sum (2^-23): within e = D 2^-23 scale sum|q k| of the true one, so a
-    weight is within 2 e.  Weights are rounded to fp16 (2^-11 relative, or 2^-25 of 2^8 times the largest), the exponential is within
+    weight is within 2 e.  Weights are rounded to fp16 with the largest at 2^6 or above: by 2^-11 of themselves or, below fp16's normal
+    numbers, by half of its step there, 2^-25, which is 2^-31 of the largest.  The exponential is within
     2^-22 of its value and 2^-23 |s log2 e| (its argument is rounded), the output is rounded to bf16 (2^-8).  Sums of
     weights and of products with values are fp32 sums in a fixed order over up to n keys, split over 16 lanes' partial sums at least:
     (n / 16 + 64) 2^-23 relative to the sum of magnitudes."""
@@ -122,7 +123,7 @@ def attend(q, data, D, page_size, table, kv_lens, q_lens, causal=True, scale=Non
                     sums = (len(s) / 16 + 64) * 2.0 ** -23
                     arg = 2.0 ** -23 * (np.abs(s).max() + abs(m)) * 1.5
                     weight = 2 * e + 2.0 ** -22 + 2 * arg + 2 * sums
-                    tol[row, h] = 2.0 ** -8 * np.abs(o) * 1.01 + (2.0 ** -11 + weight) * (p @ np.abs(vh)) + len(s) * 2.0 ** -33 / l * np.abs(vh).max() + 1e-30
+                    tol[row, h] = 2.0 ** -8 * np.abs(o) * 1.01 + (2.0 ** -11 + weight) * (p @ np.abs(vh)) + len(s) * 2.0 ** -31 / l * np.abs(vh).max() + 1e-30
                     off = 0.0 if k_offset is None else D * 2.0 ** -23 * scale * float(np.abs(x) @ np.abs(k_offset[h // g].double().numpy()))
                     ltol[row, h] = weight + 2.0 ** -21 * (abs(lse[row, h]) + abs(m) + abs(shift)) + off
             row += 1

@@ -306,6 +306,34 @@ def test_several_tokens(kv_lens, q_lens, Hq, H, D, page, causal):
     check(q, cache, table, kv_lens, q_lens, causal=causal)
 
 
+@pytest.mark.parametrize("kv_lens,q_lens,Hq,H,D", [
+    ([129, 0, 1000, 256], [1] * 4, 8, 2, 128), ([640], [1], 3, 1, 64), ([1153, 300], [6, 2], 4, 1, 128), ([2000, 90, 1], [5, 3, 4], 5, 1, 64),
+    ([700, 1200], [8, 5], 4, 2, 64), ([1100], [4], 4, 1, 128)])
+def test_keys_of_an_item_over_a_few_ctas(kv_lens, q_lens, Hq, H, D):
+    """Two to eleven blocks of keys over two, four or eight CTAs, some of which then have none."""
+    g = gen(sum(kv_lens) + Hq)
+    cache, table = make_cache(g, kv_lens, H, D, 64, offset=True)
+    check(normal(g, sum(q_lens), Hq, D).to(DEV), cache, table, kv_lens, q_lens)
+
+
+@pytest.mark.parametrize("tokens,D", [(1, 128), (1, 64), (5, 128), (6, 64)])
+def test_more_items_than_fit_at_once(tokens, D):
+    g = gen(21 + tokens)
+    kv_lens = torch.randint(400, (60,), generator=g).tolist()
+    kv_lens[7] = 520
+    cache, table = make_cache(g, kv_lens, 4, D, 16)
+    q_lens = torch.randint(tokens + 1, (60,), generator=g).tolist() if tokens > 1 else [1] * 60
+    q_lens[5] = tokens
+    check(normal(g, sum(q_lens), 16, D).to(DEV), cache, table, kv_lens, q_lens)
+
+
+@pytest.mark.parametrize("tokens,D", [(2, 128), (5, 128), (6, 64), (8, 64)])
+def test_long_rows_of_several_tokens(tokens, D):
+    g = gen(31 + tokens)
+    cache, table = make_cache(g, [9001, 130], 1, D, 128, offset=True)
+    check(normal(g, 2 * tokens, 4, D).to(DEV), cache, table, [9001, 130], [tokens, tokens])
+
+
 def test_many_ranges_of_keys():
     g = gen(9)
     kv_lens = [40001, 5, 20000]
