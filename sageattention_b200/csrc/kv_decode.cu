@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
 
   auto group_of = [&](int row) { return P.group == 1 ? row : (int)__umulhi((uint32_t)row, P.group_inverse); };       // row / group
 
-  // ---- a part of an item: `take` blocks from `block` on
-  auto item_part = [&](const KvSeq& seq, int b, int h, int tile, int block, int take, int blocks) {
+  // ---- a part of an item: `take` blocks from `block` on (`unit`: the number of its first unit)
+  auto item_part = [&](const KvSeq& seq, int b, int h, int tile, int block, int take, int blocks, int unit) {
     const int bh = b * A.Hkv + h;
     const int rows = seq.q_len * P.group, row0 = tile * kRows;
     const int last_row = min(rows, row0 + kRows) - 1;
@@ -402,6 +402,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
+    if (!kCluster && head_of_item && threadIdx.x == 0) P.item_start[(int64_t)bh * P.tiles + tile] = unit;
+
     // ---- join the four warps
     __syncthreads();
     float* const o_s = reinterpret_cast<float*>(sm + L::o);               // [warp][row][D + 4]
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
     const int rows = seq.q_len * P.group, row0 = tile * kRows;
     if (row0 >= rows) return;              // (the whole cluster)
     const int blocks = blocks_of(seq), per = (blocks + P.parts - 1) / P.parts, block = min(part * per, blocks);
-    item_part(seq, b, h, tile, block, min(per, blocks - block), blocks);
+    item_part(seq, b, h, tile, block, min(per, blocks - block), blocks, 0);
     cluster_sync();
     // rows dealt out to the CTAs' warps, parts in the order of the keys
     constexpr int kPer = D / 32;
@@ -561,8 +563,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
         continue;
       }
       const int item = rest / blocks, block = rest - item * blocks, take = min(blocks - block, unit_end - unit), h = item / tiles, tile = item - h * tiles;
-      item_part(seq, b, h, tile, block, take, blocks);
-      if (block == 0 && threadIdx.x == 0) P.item_start[(int64_t)(b * A.Hkv + h) * P.tiles + tile] = unit;
+      item_part(seq, b, h, tile, block, take, blocks, unit);
       unit += take;
       rest += take;
       __syncthreads();                       // the ring is the next item's
