@@ -9,7 +9,8 @@ namespace sage3 {
 // Block tables.  With have = ceil(before / ps), need = ceil((before + new) / ps) - have and their exclusive sums, new page number e of
 // the step belongs to the request that a search in the sums finds, and so does token t.  One launch: every CTA scans all requests
 // (8 bytes each, from L2) into shared memory and then takes its share of pages and tokens, so that one request with a long
-// prompt costs no more than many with short ones.  Bound by the launch: 48 requests 2.6 us, 700 requests and 1e5 tokens 4 us.
+// prompt costs no more than many with short ones.  Bound by its latencies, a chain of loads and barriers: 48 requests of one
+// token 3.0 us, 700 requests and 1e5 tokens 8.7 us.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTableThreads = 256;
 
@@ -22,6 +23,9 @@ __device__ __forceinline__ int find_owner(const int* start, int n, int x) {
   }
   return lo;
 }
+
+// sum of two counts, held below 2^31 (still associative, so the prefix sums stay sorted whatever the lengths)
+__device__ __forceinline__ int add_sat(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7fffffffu); }
 
 __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const KvTablesArgs A) {
   extern __shared__ int sm[];
@@ -39,22 +43,23 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const KvTab
   int tokens = 0, wanted = 0, before, fresh, have, need;
   for (int i = first; i < last; ++i) {
     lengths(i, before, fresh, have, need);
-    tokens += fresh; wanted += need;
+    tokens = add_sat(tokens, fresh); wanted = add_sat(wanted, need);
   }
   int2 incl = make_int2(tokens, wanted);
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const int x = __shfl_up_sync(0xffffffffu, incl.x, d), y = __shfl_up_sync(0xffffffffu, incl.y, d);
-    if ((t & 31) >= d) { incl.x += x; incl.y += y; }
+    if ((t & 31) >= d) { incl.x = add_sat(incl.x, x); incl.y = add_sat(incl.y, y); }
   }
   if ((t & 31) == 31) warp_sum[t >> 5] = incl;
   __syncthreads();
-  int2 run = make_int2(incl.x - tokens, incl.y - wanted);
-  for (int w = 0; w < (t >> 5); ++w) { run.x += warp_sum[w].x; run.y += warp_sum[w].y; }
+  int2 run = make_int2(__shfl_up_sync(0xffffffffu, incl.x, 1), __shfl_up_sync(0xffffffffu, incl.y, 1));
+  if ((t & 31) == 0) run = make_int2(0, 0);
+  for (int w = 0; w < (t >> 5); ++w) { run.x = add_sat(run.x, warp_sum[w].x); run.y = add_sat(run.y, warp_sum[w].y); }
   for (int i = first; i < last; ++i) {
     lengths(i, before, fresh, have, need);
     cu[i] = run.x; pages[i] = run.y;
-    run.x += fresh; run.y += need;
+    run.x = add_sat(run.x, fresh); run.y = add_sat(run.y, need);
     if (blockIdx.x == 0) A.kv_lens[i] = before + fresh;
   }
   if (t == kTableThreads - 1) {           // (the last thread's range ends at B, or is empty there)
@@ -67,24 +72,24 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const KvTab
   }
   const int at = blockIdx.x * kTableThreads + t, step = gridDim.x * kTableThreads;
   // new entries; the tokens below take those from the free list too, so nobody reads what is written here
-  for (int e = at; e < pages[A.B]; e += step) {
-    const int i = find_owner(pages, A.B, e);
+  for (int64_t e = at; e < pages[A.B]; e += step) {
+    const int i = find_owner(pages, A.B, (int)e);
     lengths(i, before, fresh, have, need);
-    const int64_t col = (int64_t)have + e - pages[i];
+    const int64_t col = have + e - pages[i];
     if (col < A.cols) A.table[i * A.table_stride + col] = e < A.num_free ? __ldg(A.free_pages + e) : -1;
   }
-  for (int x = at; x < A.num_tokens; x += step) {
+  for (int64_t x = at; x < A.num_tokens; x += step) {
     int64_t slot = -1;
     int pos = 0;
     if (x < cu[A.B]) {
-      const int i = find_owner(cu, A.B, x);
+      const int i = find_owner(cu, A.B, (int)x);
       lengths(i, before, fresh, have, need);
-      pos = before + x - cu[i];
+      pos = (int)(before + x - cu[i]);
       const int col = pos / A.page_size;
       int page = -1;
       if (col < A.cols) {
         if (col < have) page = A.table[i * A.table_stride + col];
-        else if (pages[i] + col - have < A.num_free) page = __ldg(A.free_pages + pages[i] + col - have);
+        else if ((int64_t)pages[i] + col - have < A.num_free) page = __ldg(A.free_pages + pages[i] + col - have);
       }
       if (page >= 0) slot = (int64_t)page * A.page_size + pos % A.page_size;
     }
@@ -110,8 +115,8 @@ cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream) {
 // takes a token's heads `span` at a time, kRows of them loaded before the first is used.
 //   y = x rsqrt(mean(x^2) + eps) w,   out = y cos - y' sin  or  y cos + y' sin,   y' the partner's (i +- R/2, or the neighbour i ^ 1)
 // What depends on the channel and the token alone, w cos and the partner's w sin, is worked out once for all heads, so a channel costs a
-// product, a fused one and the row's factor (975 -> 300 instructions for 8 rows of 128; N32760 H40/40 412 -> 226 us).  All in fp32, one rounding
-// to bf16.  To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
+// product, a fused one and the row's factor (490 instructions for 8 rows of 128, half of what it was; N32760, 40 heads of 128 in q and k 412
+// -> 227 us, 5.9 TB/s, neighbours paired; halves 237).  All in fp32, one rounding to bf16.  To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
 // e4m3(max|x| / 6) over the two lanes of a block, code = e2m1(x / scale).  Bound by DRAM.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTokenThreads = 256;
