@@ -82,8 +82,21 @@ def _check_b200(device, tensor):
 
 
 def _strides(x):
-    """(stride_h, stride_n) of [tokens, heads, head_dim]"""
-    return x.stride(1), x.stride(0)
+    """(stride_h, stride_n) of [tokens, heads, head_dim]; where there is but one, its stride says nothing"""
+    n, h, _ = x.shape
+    return x.stride(1) if h != 1 else 0, x.stride(0) if n != 1 else 0
+
+
+def _strides4(x, tensor_layout):
+    """(stride_b, stride_h, stride_n), likewise"""
+    B, H, N, _, *strides = _as_bhnd_strides(x, tensor_layout)
+    return [s if n != 1 else 0 for s, n in zip(strides, (B, H, N))]
+
+
+def _check_numbers(**numbers):
+    """A plan is found by these: a tensor would be found by its identity, whatever it has come to hold."""
+    for name, x in numbers.items():
+        _require(not isinstance(x, torch.Tensor), f"{name} must be a number, not a tensor")
 
 
 def _run(fn, struct, device, where):
@@ -108,7 +121,10 @@ class FP4KVCache:
     calibrated beforehand, take the place of K smoothing (``sageattn4/api.py:184``), which would need all keys at once.  Softmax does
     not see it; :func:`sageattn_kvcache` puts it back into the log-sum-exp, :meth:`read` into the keys."""
 
-    __slots__ = ("data", "num_pages", "num_kv_heads", "page_size", "head_dim", "k_offset", "device", "_key", "_struct", "_ref")
+    __slots__ = ("_data", "num_pages", "num_kv_heads", "page_size", "head_dim", "_k_offset", "device", "_key", "_struct", "_ref")
+
+    data = property(lambda self: self._data)                         # (the struct has their pointers: not to be exchanged)
+    k_offset = property(lambda self: self._k_offset)
 
     def __init__(self, data: torch.Tensor, head_dim: int, page_size: int = 64, k_offset: Optional[torch.Tensor] = None):
         if page_size not in _PAGE_SIZES:
@@ -129,7 +145,7 @@ class FP4KVCache:
             offset = k_offset.data_ptr()
         if (pointer | (offset or 0)) & 15:
             raise ValueError("data and k_offset must start on a 16-byte boundary")
-        self.data, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim, self.k_offset = data, pages, heads, page_size, head_dim, k_offset
+        self._data, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim, self._k_offset = data, pages, heads, page_size, head_dim, k_offset
         self.device = device
         self._key = (pages, heads, head_dim, page_size, device, offset is None)
         self._struct = _lib.KvCache(pointer, pages, heads, page_size, head_dim, 64 if head_dim <= 64 else 128, offset)
@@ -189,6 +205,7 @@ class FP4KVCache:
         _check_bf16(k, v)
         _require(k.dim() == 3 and k.shape == v.shape and k.shape[1:] == (self.num_kv_heads, self.head_dim),
                  f"k and v must be [tokens, {self.num_kv_heads}, {self.head_dim}]")
+        _require(k.shape[0] < 2 ** 31 - 64, "too many tokens for one call")
         _require(k.device == v.device == self.device, "k, v and the cache must be on one device")
         _check_ids("slots", slots, torch.int64, (k.shape[0],), self.device)
         _check_rows(k, v)
@@ -214,7 +231,7 @@ def build_block_tables(lens_before: torch.Tensor, lens_new: torch.Tensor, block_
     ``block_table``: int32 ``[B, columns]``, updated in place: entry j of a request is the page of its tokens ``j * page_size ...``; entries
     of pages that the step begins are taken from the front of ``free_pages`` (int32 ``[F]``), request by request.  ``num_tokens``: how many
     entries ``positions`` and ``slots`` get, the sum of ``lens_new`` or more (a padded batch); behind the last token slots are -1 and
-    positions 0.  Nothing is read back: where the free pages or the columns do not suffice, table entries and slots are -1, and
+    positions 0.  Sums of lengths stop at 2^31 - 1.  Nothing is read back: where the free pages or the columns do not suffice, table entries and slots are -1, and
     ``pages_taken`` says how many pages the step wanted."""
     key = ("kv_tables", _sig(lens_before), free_pages.shape, block_table.shape, block_table.stride(), page_size, num_tokens)
     plan = _plans.get(key)
@@ -235,6 +252,7 @@ def build_block_tables(lens_before: torch.Tensor, lens_new: torch.Tensor, block_
 
 
 def _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_tokens) -> _Plan:
+    _check_numbers(page_size=page_size, num_tokens=num_tokens)
     _require(lens_before.dim() == 1 and lens_before.shape[0] > 0, "lens_before must be [requests]")
     B, dev = lens_before.shape[0], lens_before.device
     _require(B <= 16384, "at most 16384 requests")
@@ -242,7 +260,7 @@ def _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_
     _require(0 <= num_tokens < 2 ** 31, "num_tokens must be a count")
     _check_ids("lens_before", lens_before, torch.int32, (B,), dev)
     _check_ids("lens_new", lens_new, torch.int32, (B,), dev)
-    _require(free_pages.dim() == 1, "free_pages must be [pages]")
+    _require(free_pages.dim() == 1 and free_pages.shape[0] < 2 ** 31, "free_pages must be [pages]")
     _check_ids("free_pages", free_pages, torch.int32, free_pages.shape, dev)
     _check_table(block_table, B, dev)
     _check_device(lens_before)
@@ -255,7 +273,7 @@ def _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_
 
 
 def _check_table(t, B, dev):
-    _require(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == B and t.shape[1] > 0, f"block_table must be int32 [{B}, columns]")
+    _require(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == B and 0 < t.shape[1] < 2 ** 31, f"block_table must be int32 [{B}, columns]")
     _require(t.device == dev, f"block_table must be on {dev}")
     _require(t.stride(1) == 1 or t.shape[1] == 1, "the rows of block_table must be contiguous")
     _require(B == 1 or t.stride(0) >= t.shape[1], "the rows of block_table must not overlap")
@@ -267,6 +285,7 @@ def _sig(t):
 
 def _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout) -> _Plan:
     """Checks, and the argument struct of sage3_kv_tokens but for pointers, outputs and cache."""
+    _check_numbers(eps=eps, adjacent_pairs=adjacent_pairs)
     _check_bf16(q, k)
     _require(q.dim() == k.dim() and q.dim() in (3, 4), "q and k must be [tokens, heads, head_dim], or 4-D in tensor_layout")
     if q.dim() == 3:
@@ -274,11 +293,13 @@ def _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent
         qs, ks = (0, *_strides(q)), (0, *_strides(k))
         where = (N,)
     else:
-        B, Hq, N, D, *qs = _as_bhnd_strides(q, tensor_layout)
-        Bk, Hkv, Nk, Dk, *ks = _as_bhnd_strides(k, tensor_layout)
+        B, Hq, N, D = _as_bhnd_strides(q, tensor_layout)[:4]
+        Bk, Hkv, Nk, Dk = _as_bhnd_strides(k, tensor_layout)[:4]
+        qs, ks = _strides4(q, tensor_layout), _strides4(k, tensor_layout)
         where = (B, N)
     _require((B, N, D) == (Bk, Nk, Dk), "q and k shapes do not match")
     _require(Hkv > 0, "k must have heads")
+    _require(B * N < 2 ** 31 - 64, "too many tokens for one call")
     _require(0 < D <= 128 and D % 8 == 0, f"Unsupported head_dim: {D} (a multiple of 8, at most 128)")
     _require(q.device == k.device, "q and k must be on one device")
     _check_rows(q, k)
@@ -315,7 +336,7 @@ def _norm_rope_plan(q, k, cos, sin, positions, q_weight, k_weight, eps, adjacent
 def _rows(x, tensor_layout):
     if x.dim() == 3:
         return _lib.Tensor(x.data_ptr(), 0, *_strides(x))
-    return _lib.Tensor(x.data_ptr(), *_as_bhnd_strides(x, tensor_layout)[4:])
+    return _lib.Tensor(x.data_ptr(), *_strides4(x, tensor_layout))
 
 
 def _norm_rope_key(name, q, k, cos, positions, q_weight, k_weight, eps, adjacent_pairs, tensor_layout, *more):
@@ -450,7 +471,7 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     if out is not None:
         _check_out(out, q)
     key = ("kvcache", q.shape, q.stride(), q.dtype, q.device, cache._key, block_table.shape, block_table.stride(), kv_lens.shape, cu_seqlens_q is None,
-           max_seqlen_q, max_seqlen_k, bool(is_causal), sm_scale)
+           max_seqlen_q, max_seqlen_k, is_causal, sm_scale)
     plan = _plans.get(key)
     if (plan is None or not _is(kv_lens, torch.int32, kv_lens.shape, plan.device) or block_table.dtype is not torch.int32 or
             block_table.device != plan.device or not (cu_seqlens_q is None or _is(cu_seqlens_q, torch.int32, plan.where, plan.device))):
@@ -483,6 +504,7 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
 
 
 def _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, is_causal, sm_scale) -> _Plan:
+    _check_numbers(max_seqlen_q=max_seqlen_q, max_seqlen_k=max_seqlen_k, is_causal=is_causal, sm_scale=sm_scale)
     _check_bf16(q)
     _require(q.dim() == 3 and q.shape[2] == cache.head_dim, f"q must be [tokens, heads, {cache.head_dim}]")
     T, Hq, _ = q.shape
@@ -502,7 +524,8 @@ def _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, 
     room = block_table.shape[1] * cache.page_size
     max_seqlen_k = room if max_seqlen_k is None else min(int(max_seqlen_k), room)
     _require(max_seqlen_k > 0, "max_seqlen_k must be positive")
-    _require(sm_scale is None or sm_scale > 0, "sm_scale must be positive")
+    _require(max_seqlen_k <= 2 ** 30 and max_seqlen_q < 2 ** 30 and T < 2 ** 31 and B < 2 ** 31, "too many tokens for one call")
+    _require(sm_scale is None or 0 < C.c_float(sm_scale).value < float("inf"), "sm_scale must be positive and finite in fp32")
     _check_rows(q)
     _check_device(q)
     plan = _Plan()

@@ -285,3 +285,39 @@ def test_a_kept_plan_does_not_let_another_tensor_through(monkeypatch):
         with pytest.raises(ValueError):
             sa.build_block_tables(**table_args(**kw))
     assert len(calls) == 4
+
+
+def test_a_cache_keeps_its_tensors():
+    c = cache()
+    with pytest.raises(AttributeError):
+        c.data = torch.zeros_like(c.data)
+    with pytest.raises(AttributeError):
+        c.k_offset = None
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(max_seqlen_q=torch.tensor(2)), "not a tensor"), (dict(max_seqlen_k=torch.tensor(20)), "not a tensor"), (dict(sm_scale=torch.tensor(0.5)), "not a tensor"),
+    (dict(sm_scale=1e-50), "sm_scale"), (dict(sm_scale=1e60), "sm_scale"), (dict(sm_scale=float("nan")), "sm_scale")])
+def test_attention_numbers(kw, match):
+    with pytest.raises(ValueError, match=match):
+        sa.sageattn_kvcache(**attention_args(**kw))
+
+
+def test_queries_beyond_the_grid():
+    with pytest.raises(ValueError, match="too many"):
+        sa.sageattn_kvcache(**attention_args(cu_seqlens_q=ints(0, 1, 2), max_seqlen_q=2 ** 30))
+
+
+def test_a_table_of_more_keys_than_32_bits_count():
+    wide = torch.zeros(attention_args()["block_table"].shape[0], 2 ** 26 + 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="too many"):
+        sa.sageattn_kvcache(**attention_args(block_table=wide))
+    with pytest.raises(ValueError, match="CUDA tensors only"):
+        sa.sageattn_kvcache(**attention_args(block_table=wide, max_seqlen_k=100))
+
+
+def test_numbers_of_tables_and_rotation():
+    with pytest.raises(ValueError, match="not a tensor"):
+        sa.build_block_tables(**table_args(num_tokens=torch.tensor(3)))
+    with pytest.raises(ValueError, match="not a tensor"):
+        sa.qk_norm_rope(**rope_args(eps=torch.tensor(1e-6)))

@@ -573,3 +573,35 @@ def test_block_tables_without_free_pages_or_tokens():
     assert t.tolist() == [[4, -1], [7, -1]] and r.slots.tolist() == [69, 70, 71, -1, -1] and r.pages_taken.tolist() == [1]
     t, r = run_tables([5, 16], [0, 0], [[4, -1], [7, -1]], [], 16, 0)
     assert r.slots.numel() == r.positions.numel() == 0 and r.kv_lens.tolist() == [5, 16] and r.cu_seqlens_q.tolist() == [0, 0, 0]
+
+
+def test_lengths_whose_sums_pass_32_bits():
+    """Lengths that no cache can hold: the sums stop below 2^31, and every write stays in the table."""
+    big = 2 ** 31 - 1
+    i32 = dict(dtype=torch.int32, device=DEV)
+    for before, new in (([0, 0, 0, 0], [big, big, big, 9]), ([big, 0, 7, 3], [big, 5, 1, 1]), ([0] * 40 + [3] * 3, [0] * 40 + [2 ** 30] * 3)):
+        B = len(before)
+        table = torch.full((B + 2, 8), 5, **i32)
+        r = sa.build_block_tables(torch.tensor(before, **i32), torch.tensor(new, **i32), table[1:-1], torch.arange(4, **i32), 128, 100)
+        fresh = [min(n, big - b) for b, n in zip(before, new)]
+        assert r.kv_lens.tolist() == [b + n for b, n in zip(before, fresh)]
+        assert r.cu_seqlens_q.tolist() == [min(sum(fresh[:i]), big) for i in range(B + 1)]
+        assert r.pages_taken.item() == min(sum(-(-(b + n) // 128) + b // -128 for b, n in zip(before, fresh)), big)
+        assert (table[0] == 5).all() and (table[-1] == 5).all()
+        places = [b + t for b, n in zip(before, fresh) for t in range(min(n, 100))][:100]
+        assert r.positions.tolist() == places + [0] * (100 - len(places))
+
+
+def test_strides_of_single_rows_and_heads_say_nothing():
+    g = gen(41)
+    cache, table = make_cache(g, [50], 1, 64, 16)
+    flat = normal(g, 1000).to(DEV)
+    q = flat.as_strided((1, 3, 64), (77, 64, 1))
+    want, lse = check(q, cache, table, [50], [1], no_cu=True)
+    one = flat.as_strided((3, 1, 64), (64, 5, 1))
+    k, v, slots = one, one, torch.arange(3, device=DEV)
+    cache.append(k, v, slots)
+    a, b = sa.qk_norm_rope(one, one.as_strided((3, 1, 64), (64, 3, 1)))
+    assert torch.equal(a, one) and torch.equal(b, one)
+    c = sa.qk_norm_rope(flat.as_strided((1, 3, 1, 64), (33, 64, 7, 1)), flat.as_strided((1, 3, 1, 64), (1, 64, 9, 1)))
+    assert torch.equal(c[0][0], one) and torch.equal(c[1][0], one)
