@@ -231,8 +231,27 @@ __device__ __forceinline__ void apply_lambda(uint32_t* r, const float* lam16) {
   r[0] = 0xff800000u;
 }
 
-// Which of the 8 pairs of a 16-key block take ex2_poly (x <= log2(6) here; its 2^-125 for a masked score is code 0, and nothing beside
-// the 6 that the block's largest value adds to its sum): 3 in 16.  Whole operator for 0 / 2 / 3 / 4 of 16 on rows of 256 key tiles
+// 2^x for two values on the FMA pipe (the special-function unit paces the softmax): x = n + r with n the nearest
+// integer, found by adding and subtracting 1.5 * 2^23, |r| <= 1/2; 2^r by a polynomial of degree 5, minimax in the
+// relative error (Remez exchange, computed for this file: 1.5e-7 with its coefficients rounded to fp32, 2.1e-7 = 2^-22.2 evaluated in
+// fp32, the error bound of ex2.approx being 2^-22); n goes into the exponent bits.  x <= log2(6) here; below -125 (a
+// masked score) the result is 2^-125: code 0, and nothing beside the 6 that the block's largest value adds to its sum.
+// So is that of a NaN, which has to reach the row sum by another way: nan_of_poly_columns.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  const auto both = [](const float v) { return make_float2(v, v); };
+  x.x = fmaxf(x.x, -125.f); x.y = fmaxf(x.y, -125.f);
+  const float2 t = fadd2(x, both(12582912.f));
+  const float2 r = ffma2(fadd2(t, both(-12582912.f)), both(-1.f), x);
+  float2 p = ffma2(r, both(0.0013276472454890609f), both(0.009675540961325169f));
+  p = ffma2(p, r, both(0.05550713092088699f));
+  p = ffma2(p, r, both(0.24022120237350464f));
+  p = ffma2(p, r, both(0.6931469440460205f));
+  p = ffma2(p, r, both(1.0000001192092896f));
+  p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
+  p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
+  return p;
+}
+// Which of the 8 pairs of a 16-key block take it: 3 in 16.  Whole operator for 0 / 2 / 3 / 4 of 16 on rows of 256 key tiles
 // (B1 H10 N32760): D=128 3.55 / 3.42 / 3.41 / 3.45 ms, D=64 3.61 / 3.37 / 3.27 / 3.54 ms - more, and the 12
 // instructions per pair cost more issue slots than the unit's cycles they save.
 __device__ constexpr bool on_fma_pipe(const int blk, const int pair) { return pair == 3 || (pair == 6 && (blk & 1)); }

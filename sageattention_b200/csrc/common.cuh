@@ -53,26 +53,6 @@ __device__ __forceinline__ float ex2_approx(float a) {
   return r;
 }
 
-// 2^x for two values on the FMA pipe (the special-function unit paces the softmax): x = n + r with n the nearest
-// integer, found by adding and subtracting 1.5 * 2^23, |r| <= 1/2; 2^r by a polynomial of degree 5, minimax in the
-// relative error (Remez exchange, computed for this function: 1.5e-7 with its coefficients rounded to fp32, 2.1e-7 = 2^-22.2 evaluated in
-// fp32, the error bound of ex2.approx being 2^-22); n goes into the exponent bits.  x < 127; below -125 (a masked
-// score) the result is 2^-125, and so it is for a NaN, which has to reach the row sum by another way.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  const auto both = [](const float v) { return make_float2(v, v); };
-  x.x = fmaxf(x.x, -125.f); x.y = fmaxf(x.y, -125.f);
-  const float2 t = fadd2(x, both(12582912.f));
-  const float2 r = ffma2(fadd2(t, both(-12582912.f)), both(-1.f), x);
-  float2 p = ffma2(r, both(0.0013276472454890609f), both(0.009675540961325169f));
-  p = ffma2(p, r, both(0.05550713092088699f));
-  p = ffma2(p, r, both(0.24022120237350464f));
-  p = ffma2(p, r, both(0.6931469440460205f));
-  p = ffma2(p, r, both(1.0000001192092896f));
-  p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
-  p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
-  return p;
-}
-
 constexpr float kNoMax = -1.0e30f;                     // row maximum where no key has been visible
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2Inv2688 = -11.392317422778762f;   // log2(1 / (448 * 6))  softmax_fused.h:33

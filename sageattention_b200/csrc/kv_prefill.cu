@@ -1,26 +1,29 @@
 // Attention of many query rows per kv head over the 4-bit cache: chunks of prompts behind cached prefixes.
 //
 // A CTA takes 256 rows (tokens times the heads of a kv head, two tiles of 128) of a (sequence, kv head) and walks tiles of 128 keys:
-//   warps 8-11   read the keys' part of the records, turn codes and scales into fp16 (exact, see kv_decode.cu) and write K
-//                tiles to shared memory, once for all 256 rows
-//   warps 12-15  the same with values.  Both tiles lie alike, rows of keys with 128-byte swizzle: K is then the K-major B operand of
-//                S = Q K^T and V the MN-major one of O += P V, so nothing is transposed
-//   warp  17     fetches the records by bulk copies
-//   warp  16     issues the tcgen05.mma kind::f16: S_t = Q_t K^T (queries from shared memory), O_t += P_t V (P from tensor memory)
-//   warps 0-3    softmax of row tile 0, a thread per row: scores from tensor memory to registers, weights back over them in fp16
+//   warp  13     fetches a tile's records by bulk copies
+//   warps 8-11   turn codes and scales into fp16 (exact, see kv_decode.cu), once for all 256 rows, and write K and V to shared memory.  Both
+//                lie alike, rows of keys with 128-byte swizzle: K is then the K-major B operand of S = Q K^T and V the MN-major one
+//                of O += P V, so nothing is transposed
+//   warp  12     issues the tcgen05.mma kind::f16: S_t = Q_t K^T (queries from shared memory), O_t += P_t V (P from tensor memory)
+//   warps 0-3    softmax of row tile 0, a thread per row: scores from tensor memory to registers, weights back to it in fp16
 //   warps 4-7    the same for row tile 1; one tile's softmax runs beside the other's MMAs
-// A row's maximum need not be its maximum (kv_attn.cuh): a thread takes the weights of 64 keys against the one that it has, and only where
-// their sum shows one too large for fp16 does it look for the maximum, rescale its row of O and take them again.  The P V of the
-// first 64 keys of a tile runs beside the softmax of the others.
+// Scores are copied whole before they are worked on, which frees their place: a tile's next ones are issued in front of its P V and are there
+// when its softmax comes for them.  A row's maximum need not be its maximum (kv_attn.cuh): a thread takes the weights of 128 keys
+// against the one that it has, and only where their sum shows one too large for fp16 does it look for the maximum, rescale its
+// row of O and take them again.  Weights are rounded to fp16 (by 2^-11 at most) for the MMA, their sum is of what they were.
 // With few items the keys are split over CTAs as well and joined by a second kernel.
 //
-// Tensor memory (512 columns): S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t takes the first 64 columns of S_t:
-// the MMAs are executed in the order of their issue, so Q_t K^T of the next key tile comes behind the P_t V that reads them.
+// What bounds it: the instructions of the two softmaxes and of the conversion, which share the SM's four issue ports (the tensor pipe is half
+// idle), and with few items per SM the last wave.  Two sequences of 2048 tokens behind 16384 keys, 32 heads of 8, D=128: 905 us, 1139 TFLOP/s
+// of the 1688 that bf16 GEMMs reach; a plain
+// form with mma.sync took 5 ms.
 //
-// Every wait on an mbarrier is bounded; where one gives up the CTA records its code in *status, waits (bounded) for its MMAs in
+// Tensor memory (512 columns): O0 [0, D), O1 [D, 2 D), S from 2 D on (128 columns; D=64: two of them), P0 [384, 448), P1 [448, 512).
+//
+// Every wait on an mbarrier is bounded; where one gives up the CTA records its code in *status, waits (bounded) for its MMAs and copies in
 // flight, frees its tensor memory and returns: 60 K stage free, 61 V stage free, 62 Q there, 63 K there, 64 V there, 65 P there, 66 scores
-// there, 67 last P V done; 68 tensor memory begins elsewhere; 69 records
-// there, 71 records read.
+// there, 67 last P V done, 69 records there, 70 scores copied, 71 records read; 68 tensor memory begins elsewhere.
 #include "kv_attn.cuh"
 
 namespace sage3 {
@@ -659,9 +662,9 @@ cudaError_t launch(const Params2& P, const Plan2& p, cudaStream_t stream) {
 
 }  // namespace
 
-// Rows per kv head from which on this kernel takes over.  kv_decode.cu turns a key's codes into fp16 once for 16 rows, this one once
-// for 256, but works on 128 rows at least.  Decode / prefill, B16 Hkv8 4096 keys: D=128 20 rows 54 / 58 us, 32 rows 57 / 58, 64 rows 93 / 59;
-// D=64 32 rows 36 / 49, 64 rows 57 / 49; B1 32768 keys, D=128: 20 rows 40 / 36, 64 rows 58 / 40.
+// Rows per kv head from which on this kernel takes over.  kv_decode.cu turns a key's codes into fp16 once for 24 (32) rows, this one once
+// for 256, but works on 128 rows at least.  Decode / prefill, 32 heads of 8, 4096 keys, us: B16 D=128 24 rows 37.8 / 51.6, 32 rows 51.7 /
+// 51.6; D=64 32 rows 31.3 / 46.3, 48 rows 41.2 / 46.3; B4 D=128 24 rows 15.8 / 23.9, 32 rows 24.8 / 23.9.
 bool kv_prefill_takes(int Hq, int Hkv, int DS, int max_q) { return (int64_t)max_q * (Hq / Hkv) > (DS == 128 ? 32 : 48); }
 
 size_t kv_prefill_workspace(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) { return plan2(B, Hq, Hkv, DS, max_q, max_k, sms).bytes; }
