@@ -12,12 +12,11 @@
 // when its softmax comes for them.  A row's maximum need not be its maximum (kv_attn.cuh): a thread takes the weights of 128 keys
 // against the one that it has, and only where their sum shows one too large for fp16 does it look for the maximum, rescale its
 // row of O and take them again.  Weights are rounded to fp16 (by 2^-11 at most) for the MMA, their sum is of what they were.
-// With few items the keys are split over CTAs as well and joined by a second kernel.
+// The items of the last round have their keys split over CTAs as well and joined by a second kernel.
 //
 // What bounds it: the instructions of the two softmaxes and of the conversion, which share the SM's four issue ports (the tensor pipe is half
-// idle), and with few items per SM the last wave.  Two sequences of 2048 tokens behind 16384 keys, 32 heads of 8, D=128: 905 us, 1139 TFLOP/s
-// of the 1688 that bf16 GEMMs reach; a plain
-// form with mma.sync took 5 ms.
+// idle).  Two sequences of 2048 tokens behind 16384 keys, 32 heads of 8, D=128: 862 us, 1196 TFLOP/s of the 1688 that bf16 GEMMs reach; a
+// plain form with mma.sync took 5 ms.
 //
 // Tensor memory (512 columns): O0 [0, D), O1 [D, 2 D), S from 2 D on (128 columns; D=64: two of them), P0 [384, 448), P1 [448, 512).
 //
@@ -55,24 +54,25 @@ struct Bar {                              // byte offsets in the barrier block, 
 
 struct Params2 {
   KvAttnArgs a;
-  int group, tiles, splits, page_shift;
+  int group, tiles, page_shift;
+  int whole, rest, splits;                // items that a CTA has alone, and those behind them, whose keys are split
   float scale_log2;
   int* status;
-  float* o_part;                          // [split, B * Hkv, tiles, 256, DS]
-  float2* ml_part;                        // [split, B * Hkv, tiles, 256]: maximum (log2) and sum
-  float* lse_add;                         // [B * Hkv, tiles, 256]
+  float* o_part;                          // [split, rest, 256, DS]
+  float2* ml_part;                        // [split, rest, 256]: maximum (log2) and sum
+  float* lse_add;                         // [rest, 256]
 };
 
 // Key tiles that the two row tiles of an item see, and a split's share of them
 struct Range {
   int n[2], first, count[2];
-  __device__ __forceinline__ Range(const KvSeq& seq, const Params2& P, int row0, int rows, int split) {
+  __device__ __forceinline__ Range(const KvSeq& seq, const Params2& P, int row0, int rows, int split, int splits) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int r0 = row0 + t * kM;
       n[t] = r0 < rows ? (seq.seen(P.a, (min(rows, r0 + kM) - 1) / P.group) + kN - 1) / kN : 0;
     }
-    const int all = max(n[0], n[1]), per = (all + P.splits - 1) / P.splits;
+    const int all = max(n[0], n[1]), per = (all + splits - 1) / splits;
     first = min(split * per, all);
 #pragma unroll
     for (int t = 0; t < 2; ++t) count[t] = max(0, min(min(first + per, all), n[t]) - first);
@@ -142,14 +142,16 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
   pdl_launch_dependents();
 
   // ---- the item: the last rows, which see the most keys, first
-  const int heads = A.B * A.Hkv, bh = blockIdx.x % heads, tile = P.tiles - 1 - (int)(blockIdx.x / heads), split = blockIdx.y;
+  const int behind = (int)blockIdx.x - P.whole, splits = behind < 0 ? 1 : P.splits, split = behind < 0 ? 0 : behind / P.rest;
+  const int item = behind < 0 ? (int)blockIdx.x : P.whole + behind - split * P.rest;
+  const int heads = A.B * A.Hkv, bh = item % heads, tile = P.tiles - 1 - item / heads;
   const int b = bh / A.Hkv, h = bh - b * A.Hkv;
   const KvSeq seq(A, b);
   const int rows = seq.q_len * P.group, row0 = tile * kItemRows;
   if (row0 >= rows) return;
-  const Range R(seq, P, row0, rows, split);
+  const Range R(seq, P, row0, rows, split, splits);
   const int steps = max(R.count[0], R.count[1]);
-  if (steps == 0 && P.splits > 1) return;                      // (the joining kernel knows)
+  if (steps == 0 && splits > 1) return;                      // (the joining kernel knows)
   const int see_any = seq.seen(A, (min(rows, row0 + kItemRows) - 1) / P.group);
   const int* const table = A.table + b * A.table_stride;
   const int key_begin = R.first * kN, key_end = min((R.first + steps) * kN, see_any);
@@ -524,11 +526,11 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
     if (fail == 0 && count > 0) fail = wait_bar<67>(bars + Bar::pv_done + 8 * t, (count - 1) & 1);
     if (fail != 0) {
       give_up(abort_s, P.status, fail);
-    } else if (P.splits == 1 || count > 0) {
+    } else if (splits == 1 || count > 0) {
       tc_fence_after();
       const float sum = l.x + l.y, inv = sum == 0.f ? 0.f : 1.0f / sum;
-      const int64_t place = ((int64_t)bh * P.tiles + tile) * kItemRows + t * kM + r;
-      const int64_t part = (int64_t)split * heads * P.tiles * kItemRows + place;
+      const int64_t place = (int64_t)(item - P.whole) * kItemRows + t * kM + r;          // (where the keys are split)
+      const int64_t part = (int64_t)split * P.rest * kItemRows + place;
       __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh;
 #pragma unroll 1
       for (int i = 0; i < D / 32; ++i) {
@@ -541,7 +543,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
           for (int x = 0; x < 32; ++x) o[x] = 0;
         }
         if (real) {
-          if (P.splits == 1) {
+          if (splits == 1) {
 #pragma unroll
             for (int x = 0; x < 32; x += 8)
               if (32 * i + x < A.D) {
@@ -557,9 +559,9 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
           }
         }
       }
-      if (real && P.splits > 1) P.ml_part[part] = make_float2(m, sum);
+      if (real && splits > 1) P.ml_part[part] = make_float2(m, sum);
       if (real && A.lse != nullptr) {
-        if (P.splits == 1) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, sum, add);
+        if (splits == 1) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, sum, add);
         else if (split == 0) P.lse_add[place] = add;
       }
     }
@@ -580,17 +582,16 @@ __global__ void __launch_bounds__(256) kv_prefill_join_kernel(const Params2 P) {
   const KvAttnArgs& A = P.a;
   const int lane = threadIdx.x & 31;
   const uint32_t id = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int in_tile = id % kItemRows, item = id / kItemRows, tile = item % P.tiles, bh = item / P.tiles;
-  if (bh >= A.B * A.Hkv) return;                                // (a whole warp; others of the CTA wait below)
+  const int in_tile = id % kItemRows, heads = A.B * A.Hkv, item = P.whole + id / kItemRows, bh = item % heads, tile = P.tiles - 1 - item / heads;
   const int b = bh / A.Hkv, h = bh - b * A.Hkv;
   const KvSeq seq(A, b);
   const int rows = seq.q_len * P.group, row = tile * kItemRows + in_tile;
   pdl_wait();                              // also where there is no row: what follows on the stream may write the first kernel's inputs
   if (row >= rows) return;
-  const Range R(seq, P, tile * kItemRows, rows, 0);
+  const Range R(seq, P, tile * kItemRows, rows, 0, P.splits);
   const int n = R.n[in_tile / kM], all = max(R.n[0], R.n[1]), per = (all + P.splits - 1) / P.splits;
   const int used = n > 0 ? (n + per - 1) / per : 0;
-  const int64_t place = (int64_t)item * kItemRows + in_tile, step = (int64_t)A.B * A.Hkv * P.tiles * kItemRows;
+  const int64_t place = id, step = (int64_t)P.rest * kItemRows;
   float m = kLowest;
   for (int s = lane; s < used; s += 32) m = fmaxf(m, P.ml_part[place + s * step].x);
 #pragma unroll
@@ -623,19 +624,30 @@ __global__ void __launch_bounds__(256) kv_prefill_join_kernel(const Params2 P) {
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct Plan2 {
-  int tiles, splits;
-  int64_t items;
+  int tiles, whole, rest, splits;
   size_t add, ml, o, bytes;               // offsets in the workspace
 };
+
+// As many items as there are SMs take as long as one, so those of the last round have their keys split over CTAs, into as many parts as
+// make it shortest by this account, in key tiles: what an item costs beside its tiles, the joining, and a sixteenth for each partial result.
+// (us, whole items -> so, 32 heads of 8, D=128: B2 1200 tokens 16384 keys 665 -> 526, 2048 tokens 911 -> 862; B1 1600 tokens 8192 keys 213 -> 187.)
+constexpr int kItemCost = 6, kJoinCost = 10;
 
 Plan2 plan2(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
   Plan2 p;
   p.tiles = (int)(((int64_t)max_q * (Hq / Hkv) + kItemRows - 1) / kItemRows);
-  p.items = (int64_t)B * Hkv * p.tiles;
-  const int64_t key_tiles = ((int64_t)max_k + kN - 1) / kN, room = sms / p.items, most = (key_tiles + 3) / 4;
-  p.splits = (int)(room < most ? room : most);
-  if (p.splits < 1) p.splits = 1;
-  const size_t rows = p.splits > 1 ? (size_t)p.items * kItemRows : 0;
+  const int items = (int)((int64_t)B * Hkv * p.tiles), key_tiles = (int)(((int64_t)max_k + kN - 1) / kN);
+  p.rest = items % sms;
+  p.whole = items - p.rest;
+  p.splits = 1;
+  int64_t best = INT64_MAX;
+  for (int n = 1; p.rest > 0 && p.rest * (n - 1) < 4 * sms && 4 * (n - 1) <= key_tiles; ++n) {
+    const int rounds = (p.rest * n + sms - 1) / sms, tiles = (key_tiles + n - 1) / n + kItemCost;
+    const int64_t cost = 16ll * rounds * tiles + (n > 1 ? 16 * kJoinCost + p.rest * n : 0);
+    if (cost < best) { best = cost; p.splits = n; }
+  }
+  if (p.splits == 1) { p.whole += p.rest; p.rest = 0; }
+  const size_t rows = (size_t)p.rest * kItemRows;
   p.add = 256;
   p.ml = p.add + align256(rows * 4);
   p.o = p.ml + align256(rows * p.splits * 8);
@@ -655,9 +667,9 @@ cudaError_t launch(const Params2& P, const Plan2& p, cudaStream_t stream) {
   if (regs_ok != cudaSuccess) return regs_ok;
   static std::atomic<uint64_t> allowed;
   if (cudaError_t e = allow_smem(kv_prefill_kernel<D>, smem, allowed); e != cudaSuccess) return e;
-  if (cudaError_t e = launch_pdl(kv_prefill_kernel<D>, dim3((unsigned)p.items, P.splits), kThreads2, smem, stream, false, P); e != cudaSuccess) return e;
-  if (P.splits == 1) return cudaGetLastError();
-  return launch_pdl(kv_prefill_join_kernel<D>, dim3((unsigned)(p.items * kItemRows / 8)), 256, 0, stream, true, P);
+  if (cudaError_t e = launch_pdl(kv_prefill_kernel<D>, dim3((unsigned)(p.whole + p.rest * p.splits)), kThreads2, smem, stream, false, P); e != cudaSuccess) return e;
+  if (p.rest == 0) return cudaGetLastError();
+  return launch_pdl(kv_prefill_join_kernel<D>, dim3((unsigned)((int64_t)p.rest * kItemRows / 8)), 256, 0, stream, true, P);
 }
 
 }  // namespace
@@ -680,7 +692,7 @@ cudaError_t launch_kv_prefill(const KvAttnArgs& a, cudaStream_t stream) {
   const Plan2 p = plan2(a.B, a.Hq, a.Hkv, a.DS, a.max_q, a.max_k, sms);
   Params2 P;
   P.a = a;
-  P.group = a.Hq / a.Hkv; P.tiles = p.tiles; P.splits = p.splits;
+  P.group = a.Hq / a.Hkv; P.tiles = p.tiles; P.whole = p.whole; P.rest = p.rest; P.splits = p.splits;
   P.scale_log2 = a.sm_scale * kLog2e;
   P.page_shift = 0;
   while ((1 << P.page_shift) < a.page_size) ++P.page_shift;

@@ -327,6 +327,14 @@ def test_more_items_than_fit_at_once(tokens, D):
     check(normal(g, sum(q_lens), 16, D).to(DEV), cache, table, kv_lens, q_lens)
 
 
+@pytest.mark.parametrize("heads,tokens,keys,D", [(150, 33, 2100, 128), (151, 49, 2300, 64)])
+def test_keys_of_the_last_round_are_split(heads, tokens, keys, D):
+    """Two and three items more than the chip has SMs."""
+    g = gen(heads)
+    cache, table = make_cache(g, [keys], heads, D, 64, offset=True)
+    check(normal(g, tokens, heads, D).to(DEV), cache, table, [keys], [tokens])
+
+
 @pytest.mark.parametrize("tokens,D", [(2, 128), (5, 128), (6, 64), (8, 64)])
 def test_long_rows_of_several_tokens(tokens, D):
     g = gen(31 + tokens)
