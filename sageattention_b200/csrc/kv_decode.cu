@@ -30,7 +30,7 @@ struct Header {                           // at the front of the workspace, for 
 struct Params {
   KvAttnArgs a;
   int group, tiles, page_shift;           // query heads per kv head; tiles of rows of the longest sequence
-  int parts;                              // CTAs of a cluster
+  int parts, ctas;                        // CTAs of a cluster; of the equal runs
   uint32_t group_inverse;                 // 2^32 / group rounded up: exact for quotients of the few rows there are
   float scale_log2;
   Header* header;
@@ -475,15 +475,21 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
     const int b = bh / A.Hkv, h = bh - b * A.Hkv;
     const KvSeq seq(A, b);
     const int rows = seq.q_len * P.group, row0 = tile * kRows;
-    if (row0 >= rows) return;              // (the whole cluster)
-    const int blocks = blocks_of(seq), per = (blocks + P.parts - 1) / P.parts, block = min(part * per, blocks);
-    item_part(seq, b, h, tile, block, min(per, blocks - block), blocks, 0);
+    // Nobody leaves before the last barrier, and barriers do not hang on what a warp has read: lengths that another stream writes meanwhile may
+    // differ from CTA to CTA, and a CTA that has gone must not be read from.
+    const bool live = __syncthreads_and(row0 < rows);
+    if (live) {
+      const int blocks = blocks_of(seq), per = (blocks + P.parts - 1) / P.parts, block = min(part * per, blocks);
+      item_part(seq, b, h, tile, block, min(per, blocks - block), blocks, 0);
+    }
+    __syncwarp();
     cluster_sync();
     // rows dealt out to the CTAs' warps, parts in the order of the keys
     constexpr int kPer = D / 32;
     const uint32_t at_o = smem_u32(sm + L::part), at_ml = smem_u32(sm + L::part_ml);
+    const bool have = lane * kPer < A.D;
 #pragma unroll 1
-    for (int row = part + P.parts * warp; row < kRows && row0 + row < rows; row += P.parts * kWarps) {
+    for (int row = part + P.parts * warp; live && row < kRows && row0 + row < rows; row += P.parts * kWarps) {
       float2 ml = make_float2(kLowest, 0.f);
       if (lane < P.parts) ml = ld_cluster(of_cta(at_ml + row * 8, lane));
       float m = ml.x;
@@ -501,6 +507,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
           l = fmaf(w, lx, l);
 #pragma unroll
           for (int k = 0; k < kPer; k += 2) {
+            if (!have) continue;           // (a load that nothing waits for could be under way when its target goes)
             const float2 v = ld_cluster(of_cta(at_o + (row * D + lane * kPer + k) * 4, x));
             acc[k] = fmaf(w, v.x, acc[k]); acc[k + 1] = fmaf(w, v.y, acc[k + 1]);
           }
@@ -509,11 +516,12 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
       const int tok = group_of(row0 + row), hq = h * P.group + row0 + row - tok * P.group;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       __nv_bfloat16* const out = (__nv_bfloat16*)A.out + (int64_t)(seq.q0 + tok) * A.o_sn + hq * A.o_sh + lane * kPer;
-      if (lane * kPer < A.D)
+      if (have)
 #pragma unroll
         for (int k = 0; k < kPer; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pack_bf16(acc[k] * inv, acc[k + 1] * inv);
       if (lane == 0 && A.lse != nullptr) A.lse[(int64_t)(seq.q0 + tok) * A.Hq + hq] = lse_of(m, l, add_s[row]);
     }
+    __syncwarp();
     cluster_sync();                        // nobody's shared memory goes while another reads it
   } else {
     // ---- this CTA's units
@@ -546,7 +554,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
     if (unit >= unit_end) return;
     if (unit >= before && unit < before + mine) {                // one of this thread's is the first
       int b = b_first, x = before;
-      for (int n_b; unit >= x + (n_b = units(b)); ++b) x += n_b;
+      for (int n_b; b + 1 < b_last && unit >= x + (n_b = units(b)); ++b) x += n_b;
       where_s[0] = b; where_s[1] = x;
     }
     __syncthreads();
@@ -587,8 +595,9 @@ __global__ void __launch_bounds__(128) kv_join_kernel(const Params P) {
   const int row = tile * kRows + row_id;
   pdl_wait();                              // also where there is no row: what follows on the stream may write the first kernel's inputs
   if (row >= seq.q_len * P.group) return;
-  const int start = P.item_start[item], per = P.header->per;
-  const int first = start / per, last = (start + blocks_of(seq) - 1) / per;
+  // (held to the parts that there are, should lengths have changed since the first kernel read them)
+  const uint32_t start = P.item_start[item], per = max(P.header->per, 1), most = P.ctas - 1;
+  const int first = min(start / per, most), last = min((start + blocks_of(seq) - 1) / per, most);
   if (first == last) return;
   // the first CTA had the item last, the others had it first
   auto place = [&](int cta) { return ((int64_t)cta * 2 + (cta == first ? 1 : 0)) * kRows + row_id; };
@@ -675,7 +684,7 @@ struct Plan {
 
 // Up to 24 (D=64: 32) rows at a time, in tiles as equal as can be; as many CTAs as fit on the chip at once, or as there are units.
 Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
-  Plan p;
+  Plan p{};
   const int64_t rows = (int64_t)max_q * (Hq / Hkv), most = DS == 64 ? 32 : 24;
   p.tiles = (int)((rows + most - 1) / most);
   p.nb = (int)((rows + 8 * p.tiles - 1) / (8 * p.tiles));
@@ -683,14 +692,15 @@ Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
   const int64_t fit = (int64_t)sms * ctas_per_sm(DS, p.nb);
   p.units = items * blocks;
   p.rows = items * 8 * p.nb;
-  // Clusters where all of them fit at once and none has far to go: up to 4 blocks per CTA, 8 where a third of the chip is had anyway (us, equal
-  // runs -> clusters, D=128: B1, 32 heads of 8, 1000 keys 6.4 -> 5.2, 4096 8.1 -> 7.6, 16384 12.8 -> 16.6; B4 1000 keys 7.7 -> 6.3, 8192
-  // 15.6 -> 13.8; B3 of 6 tokens 4096 keys 20.0 -> 15.8).  Longer ones, and ragged ones of more keys, are better off in equal runs; one
-  // block needs no joining (100 keys 4.1 -> 4.6).
-  p.parts = 2;
-  while (p.parts < blocks && p.parts < kMostParts) p.parts *= 2;
-  if (blocks < 2 || items * p.parts > fit || blocks > (3 * items * p.parts >= fit ? 8 : 4) * p.parts) p.parts = 0;
   p.ctas = p.units < fit ? p.units : fit;
+  // Clusters, as large as all of them fit at once, where no CTA has more than 16 blocks to go through, or more than 7 above an equal share of
+  // all (us, equal runs -> clusters, 32 heads of 8, D=128: one token of B1 1000 keys 6.4 -> 5.2, B12 4096 21.0 -> 16.9, B32 2048 23.7 -> 20.6, up to 2048
+  // 20.0 -> 17.1; 4 tokens of B16 4096 34.3 -> 29.7, up to 4096 38 -> 29; 6 tokens of B16 up to 4096 53 -> 33.  Beyond: B1 16384 12.8 -> 16.6, B20
+  // up to 8192 31 -> 36.)  One block needs no joining (100 keys 4.1 -> 4.6).
+  p.parts = kMostParts;
+  while (p.parts > 1 && (items * p.parts > fit || p.parts >= 2 * blocks)) p.parts /= 2;
+  const int64_t longest = (blocks + p.parts - 1) / p.parts;
+  if (p.parts == 1 || longest > 16 || (longest - 7) * fit > p.units) p.parts = 0;
   p.starts = 256;
   p.adds = p.starts + align256(items * 4);
   p.ml = p.adds + align256(items * 8 * p.nb * 4);
@@ -741,7 +751,7 @@ cudaError_t launch_kv_decode(const KvAttnArgs& a, cudaStream_t stream) {
   P.group = a.Hq / a.Hkv; P.tiles = p.tiles;
   P.group_inverse = (uint32_t)(0xffffffffu / (uint32_t)P.group) + 1;
   P.scale_log2 = a.sm_scale * kLog2e;
-  P.parts = p.parts;
+  P.parts = p.parts; P.ctas = (int)p.ctas;
   P.page_shift = 0;
   while ((1 << P.page_shift) < a.page_size) ++P.page_shift;
   char* const w = (char*)a.workspace;

@@ -148,10 +148,10 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
   const int b = bh / A.Hkv, h = bh - b * A.Hkv;
   const KvSeq seq(A, b);
   const int rows = seq.q_len * P.group, row0 = tile * kItemRows;
-  if (row0 >= rows) return;
   const Range R(seq, P, row0, rows, split, splits);
   const int steps = max(R.count[0], R.count[1]);
-  if (steps == 0 && splits > 1) return;                      // (the joining kernel knows)
+  // no rows, or no keys among a split's (the joining kernel knows); as one, whatever a warp has read of lengths that another stream writes meanwhile
+  if (!__syncthreads_and(row0 < rows && (steps > 0 || splits == 1))) return;
   const int see_any = seq.seen(A, (min(rows, row0 + kItemRows) - 1) / P.group);
   const int* const table = A.table + b * A.table_stride;
   const int key_begin = R.first * kN, key_end = min((R.first + steps) * kN, see_any);

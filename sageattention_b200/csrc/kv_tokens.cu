@@ -71,12 +71,13 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const KvTab
     if (t == 0) A.taken[0] = pages[A.B];
   }
   const int at = blockIdx.x * kTableThreads + t, step = gridDim.x * kTableThreads;
-  // new entries; the tokens below take those from the free list too, so nobody reads what is written here
+  // (Indexes are held to their arrays from both sides: lengths that another stream writes meanwhile may differ between the passes.)
+  // New entries; the tokens below take those from the free list too, so nobody reads what is written here
   for (int64_t e = at; e < pages[A.B]; e += step) {
     const int i = find_owner(pages, A.B, (int)e);
     lengths(i, before, fresh, have, need);
     const int64_t col = have + e - pages[i];
-    if (col < A.cols) A.table[i * A.table_stride + col] = e < A.num_free ? __ldg(A.free_pages + e) : -1;
+    if ((uint64_t)col < (uint64_t)A.cols) A.table[i * A.table_stride + col] = e < A.num_free ? __ldg(A.free_pages + e) : -1;
   }
   for (int64_t x = at; x < A.num_tokens; x += step) {
     int64_t slot = -1;
@@ -87,9 +88,10 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const KvTab
       pos = (int)(before + x - cu[i]);
       const int col = pos / A.page_size;
       int page = -1;
-      if (col < A.cols) {
+      if ((uint32_t)col < (uint32_t)A.cols) {
+        const int64_t e = (int64_t)pages[i] + col - have;
         if (col < have) page = A.table[i * A.table_stride + col];
-        else if ((int64_t)pages[i] + col - have < A.num_free) page = __ldg(A.free_pages + pages[i] + col - have);
+        else if ((uint64_t)e < (uint64_t)A.num_free) page = __ldg(A.free_pages + e);
       }
       if (page >= 0) slot = (int64_t)page * A.page_size + pos % A.page_size;
     }
