@@ -91,8 +91,8 @@ constexpr int ctas_per_sm(int D, int NB) { return NB == 1 ? 4 : NB == 2 ? 3 : D 
 // The work: an item is a (sequence, kv head, tile of rows), a unit one of its blocks of 128 keys.  All units, in this order, are dealt out in
 // equal runs, so that ragged batches and single long sequences fill the chip alike; a CTA's run may end inside an item and go on to
 // others.  Only its first and its last item can be shared with other CTAs: two places for partial results each.
-// kCluster, for little work: a cluster of CTAs has an item, and its parts are joined through their shared memory; there is nothing to
-// look up in front and no second kernel.
+// kCluster, where no item is long beside the others (see plan): a cluster of CTAs has an item, and its parts are joined through their
+// shared memory; there is nothing to look up in front and no second kernel.
 template <int D, int NB, bool kCluster>   // stored head dim, 8-row blocks
 __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_kernel(const Params P) {
   using Rec = KvRecord<D>;
@@ -693,14 +693,16 @@ Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
   p.units = items * blocks;
   p.rows = items * 8 * p.nb;
   p.ctas = p.units < fit ? p.units : fit;
-  // Clusters, as large as all of them fit at once, where no CTA has more than 16 blocks to go through, or more than 7 above an equal share of
-  // all (us, equal runs -> clusters, 32 heads of 8, D=128: one token of B1 1000 keys 6.4 -> 5.2, B12 4096 21.0 -> 16.9, B32 2048 23.7 -> 20.6, up to 2048
-  // 20.0 -> 17.1; 4 tokens of B16 4096 34.3 -> 29.7, up to 4096 38 -> 29; 6 tokens of B16 up to 4096 53 -> 33.  Beyond: B1 16384 12.8 -> 16.6, B20
-  // up to 8192 31 -> 36.)  One block needs no joining (100 keys 4.1 -> 4.6).
+  // A cluster (or a CTA) per item or equal runs?  Clusters are as large as all of them fit at once; a CTA's way through the keys must not be
+  // long beside an equal share of all of them, nor the last round of CTAs nearly empty.  us, equal runs -> clusters, 32 heads of 8, D=128, "~":
+  // lengths up to that.  One token: B1 1000 keys 6.4 -> 5.2, B12 4096 21.0 -> 16.9, B32 ~2048 20.0 -> 17.1, B64 ~1000 20.9 -> 16.8, B256 ~1000
+  // 66.8 -> 46.6, B128 4096 112.5 -> 104.2; 4 tokens: B16 ~4096 38 -> 29, B128 ~1000 72.6 -> 45.1; 6 tokens: B16 ~4096 53 -> 33.
+  // What the rule leaves to equal runs: B1 16384 12.8 -> 16.6, B20 ~8192 31 -> 36, B40 ~8192 47 -> 76.  One block needs no joining (4.1 -> 4.6).
   p.parts = kMostParts;
   while (p.parts > 1 && (items * p.parts > fit || p.parts >= 2 * blocks)) p.parts /= 2;
   const int64_t longest = (blocks + p.parts - 1) / p.parts;
-  if (p.parts == 1 || longest > 16 || (longest - 7) * fit > p.units) p.parts = 0;
+  const bool clusters = items <= fit ? longest <= 16 && (longest - 7) * fit <= p.units : longest <= 32 && 10 * items >= 13 * fit;
+  if (blocks < 2 || !clusters) p.parts = 0;
   p.starts = 256;
   p.adds = p.starts + align256(items * 4);
   p.ml = p.adds + align256(items * 8 * p.nb * 4);
