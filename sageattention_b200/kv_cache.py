@@ -233,13 +233,16 @@ def build_block_tables(lens_before: torch.Tensor, lens_new: torch.Tensor, block_
     entries ``positions`` and ``slots`` get, the sum of ``lens_new`` or more (a padded batch); behind the last token slots are -1 and
     positions 0.  Sums of lengths stop at 2^31 - 1.  Nothing is read back: where the free pages or the columns do not suffice, table entries and slots are -1, and
     ``pages_taken`` says how many pages the step wanted."""
-    key = ("kv_tables", _sig(lens_before), free_pages.shape, block_table.shape, block_table.stride(), page_size, num_tokens)
+    # (the free pages and the tokens are other ones in every step: not part of the key)
+    key = ("kv_tables", _sig(lens_before), block_table.shape, block_table.stride(), page_size)
     plan = _plans.get(key)
-    if (plan is None or not _is(lens_new, torch.int32, plan.where, plan.device) or not _is(free_pages, torch.int32, plan.rows, plan.device) or
-            block_table.dtype is not torch.int32 or block_table.device != plan.device):
+    if (plan is None or not _is(lens_new, torch.int32, plan.where, plan.device) or not _is(free_pages, torch.int32, free_pages.shape, plan.device) or
+            free_pages.dim() != 1 or block_table.dtype is not torch.int32 or block_table.device != plan.device or
+            type(num_tokens) is not int or not 0 <= num_tokens < 2 ** 31 or free_pages.shape[0] >= 2 ** 31):
         plan = _keep_plan(key, _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_tokens))
     dev, a = plan.device, _lib.KvTablesArgs.from_buffer_copy(plan.struct)
-    B, n = a.B, a.num_tokens
+    B, n = a.B, int(num_tokens)
+    a.num_free, a.num_tokens = free_pages.shape[0], n
     # one allocation for all of int32
     ints = lens_new.new_empty(2 * B + 2 + n)
     kv_lens, cu, taken, positions = torch.split_with_sizes(ints, (B, B + 1, 1, n))
@@ -265,10 +268,9 @@ def _plan_tables(lens_before, lens_new, block_table, free_pages, page_size, num_
     _check_table(block_table, B, dev)
     _check_device(lens_before)
     plan = _Plan()
-    plan.device, plan.where, plan.rows = dev, lens_before.shape, free_pages.shape
+    plan.device, plan.where = dev, lens_before.shape
     a = plan.struct = _lib.KvTablesArgs()
-    a.row_stride, a.B, a.columns, a.num_free, a.page_size, a.num_tokens = (
-        max(block_table.stride(0), block_table.shape[1]), B, block_table.shape[1], free_pages.shape[0], page_size, int(num_tokens))
+    a.row_stride, a.B, a.columns, a.page_size = max(block_table.stride(0), block_table.shape[1]), B, block_table.shape[1], page_size
     return plan
 
 
@@ -470,13 +472,16 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where one of their bounded waits gave up."""
     if out is not None:
         _check_out(out, q)
+    # (what the launch is made for goes by blocks of 128 keys: a plan lasts for as many steps)
     key = ("kvcache", q.shape, q.stride(), q.dtype, q.device, cache._key, block_table.shape, block_table.stride(), kv_lens.shape, cu_seqlens_q is None,
-           max_seqlen_q, max_seqlen_k, is_causal, sm_scale)
+           max_seqlen_q, None if max_seqlen_k is None else -(-max_seqlen_k // 128), is_causal, sm_scale)
     plan = _plans.get(key)
     if (plan is None or not _is(kv_lens, torch.int32, kv_lens.shape, plan.device) or block_table.dtype is not torch.int32 or
             block_table.device != plan.device or not (cu_seqlens_q is None or _is(cu_seqlens_q, torch.int32, plan.where, plan.device))):
         plan = _keep_plan(key, _plan_attention(q, cache, block_table, kv_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, is_causal, sm_scale))
     dev, a = plan.device, _lib.KvAttentionArgs.from_buffer_copy(plan.struct)
+    if max_seqlen_k is not None:
+        a.max_seqlen_k = min(int(max_seqlen_k), a.columns * cache.page_size)
     if out is None:
         out = torch.empty_like(q)                                    # (whose strides the plan has)
     else:

@@ -308,7 +308,7 @@ def test_several_tokens(kv_lens, q_lens, Hq, H, D, page, causal):
 
 @pytest.mark.parametrize("kv_lens,q_lens,Hq,H,D", [
     ([129, 0, 1000, 256], [1] * 4, 8, 2, 128), ([640], [1], 3, 1, 64), ([1153, 300], [6, 2], 4, 1, 128), ([2000, 90, 1], [5, 3, 4], 5, 1, 64),
-    ([700, 1200], [8, 5], 4, 2, 64), ([1100], [4], 4, 1, 128)])
+    ([700, 1200], [8, 5], 4, 2, 64), ([1100], [4], 4, 1, 128), ([500, 700], [3, 1], 6, 2, 96), ([900], [2], 2, 1, 8), ([600, 5], [1, 1], 4, 4, 40)])
 def test_keys_of_an_item_over_a_few_ctas(kv_lens, q_lens, Hq, H, D):
     """Two to eleven blocks of keys over two, four or eight CTAs, some of which then have none."""
     g = gen(sum(kv_lens) + Hq)
@@ -613,3 +613,25 @@ def test_strides_of_single_rows_and_heads_say_nothing():
     assert torch.equal(a, one) and torch.equal(b, one)
     c = sa.qk_norm_rope(flat.as_strided((1, 3, 1, 64), (33, 64, 7, 1)), flat.as_strided((1, 3, 1, 64), (1, 64, 9, 1)))
     assert torch.equal(c[0][0], one) and torch.equal(c[1][0], one)
+
+
+def test_one_plan_for_lengths_of_a_block_and_for_any_free_list():
+    """Bounds that grow from step to step are held to, and so is each free list, though nothing is looked up anew."""
+    g = gen(51)
+    cache, table = make_cache(g, [300, 200], 2, 64, 16)
+    q = normal(g, 2, 4, 64).to(DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    lens, tab = torch.tensor([300, 200], **i32), table.to(DEV)
+    for bound in (257, 258, 299, 300, 384, 200, 10 ** 6):
+        n = [min(300, bound), min(200, bound)]
+        a = sa.sageattn_kvcache(q, cache, tab, lens, max_seqlen_k=bound)
+        b = sa.sageattn_kvcache(q, cache, tab, torch.tensor(n, **i32))
+        want, _, tol, _ = R.attend(q.cpu(), cache.data.cpu().numpy(), 64, 16, table.tolist(), n, [1, 1])
+        for x in (a, b):
+            assert (np.abs(x.double().cpu().numpy() - want) <= tol).all()
+    for free, tokens in (([7, 8, 9], 4), ([8], 4), ([], 5), ([5, 6, 7, 8], 3)):
+        t = torch.full((1, 4), -7, **i32)
+        r = sa.build_block_tables(torch.tensor([0], **i32), torch.tensor([3], **i32), t, torch.tensor(free, **i32), 16, tokens)
+        page = free[0] if free else -1
+        assert t.tolist() == [[page, -7, -7, -7]] and r.positions.tolist() == [0, 1, 2] + [0] * (tokens - 3)
+        assert r.slots.tolist() == [page * 16 + i if free else -1 for i in range(3)] + [-1] * (tokens - 3)
