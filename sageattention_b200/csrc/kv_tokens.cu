@@ -118,7 +118,7 @@ cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream) {
 //   y = x rsqrt(mean(x^2) + eps) w,   out = y cos - y' sin  or  y cos + y' sin,   y' the partner's (i +- R/2, or the neighbour i ^ 1)
 // What depends on the channel and the token alone, w cos and the partner's w sin, is worked out once for all heads, so a channel costs a
 // product, a fused one and the row's factor (490 instructions for 8 rows of 128, half of what it was; N32760, 40 heads of 128 in q and k 412
-// -> 227 us, 5.9 TB/s, neighbours paired; halves 237).  All in fp32, one rounding to bf16.  To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
+// -> 227 us, 5.9 TB/s, neighbours paired; halves 240).  All in fp32, one rounding to bf16.  To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
 // e4m3(max|x| / 6) over the two lanes of a block, code = e2m1(x / scale).  Bound by DRAM.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTokenThreads = 256;
@@ -166,6 +166,20 @@ __global__ void __launch_bounds__(kTokenThreads, 4) kv_tokens_kernel(const KvTok
     slot = __ldg(A.slots + token);
     if (slot < 0 || slot >= A.num_slots) slot = -1;
   }
+
+  // ---- the first rows on their way, beside what they are multiplied by
+  const __nv_bfloat16* from = src + (h0 + sub) * in.sh;
+  const int64_t from_step = kPerPass * in.sh;
+  uint4 x[kPasses];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      x[p] = make_uint4(0, 0, 0, 0);
+      if (have && first + p * kPerPass + sub < h1) x[p] = __ldg(reinterpret_cast<const uint4*>(from));
+      from += from_step;
+    }
+  };
+  load(h0);
 
   // ---- what the channels of this token are multiplied by: themselves (own), and their partners (other)
   const bool normed = what != 2 && A.weight[what] != nullptr, turned = what != 2 && l * 8 < A.rot, change = what != 2 && (normed || A.rot > 0);
@@ -238,19 +252,11 @@ __global__ void __launch_bounds__(kTokenThreads, 4) kv_tokens_kernel(const KvTok
   uint8_t* const base = A.data + page * A.Hkv * head_bytes + in_page / 16 * Rec::kBytes;
   const int code_at = what == 1 ? Rec::key(t, l * 8) : Rec::value(t, l * 8), scale_at = what == 1 ? Rec::key_scale(t, l >> 1) : Rec::value_scale(t, l >> 1);
 
-  const __nv_bfloat16* from = src + (h0 + sub) * in.sh;
-  const int64_t from_step = kPerPass * in.sh, to_step = kPerPass * out.sh;
+  const int64_t to_step = kPerPass * out.sh;
   __nv_bfloat16* to = writes ? (__nv_bfloat16*)out.ptr + b * out.sb + n * out.sn + (h0 + sub) * out.sh + l * 8 : nullptr;
 #pragma unroll 1
   for (int first = h0; first < h1; first += kRows) {
-    uint4 x[kPasses];
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int h = first + p * kPerPass + sub;
-      x[p] = make_uint4(0, 0, 0, 0);
-      if (have && h < h1) x[p] = __ldg(reinterpret_cast<const uint4*>(from));
-      from += from_step;
-    }
+    if (first != h0) load(first);
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int h = first + p * kPerPass + sub;
@@ -317,8 +323,9 @@ cudaError_t launch_kv_tokens(KvTokensArgs a, cudaStream_t stream) {
   if (cudaError_t e = sm_count(&sms); e != cudaSuccess) return e;
   const int rows = a.DS == 128 ? 8 : 16;                        // kRows
   const int most = a.Hq > a.Hkv ? a.Hq : a.Hkv, tokens = a.B * a.N;
-  // as many heads per warp as leave two rounds of warps; the angles and weights of a token are then fetched once for them
-  const int64_t want = 64ll * sms;
+  // as many heads per warp as leave a round of warps, for which the angles and weights of a token are then fetched once (2000 tokens, 32 + 8
+  // heads of 128: two rounds 11.7 us, one 10.6, half a one 12.0)
+  const int64_t want = 32ll * sms;
   a.span = rows;
   while (a.span < most && (int64_t)tokens * ((a.Hq + 2 * a.span - 1) / (2 * a.span) + (a.Hkv + 2 * a.span - 1) / (2 * a.span)) >= want) a.span *= 2;
   const int groups = (a.Hq + a.span - 1) / a.span + (a.Hkv + a.span - 1) / a.span * (a.v != nullptr ? 2 : 1);
