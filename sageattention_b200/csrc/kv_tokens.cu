@@ -117,7 +117,7 @@ cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream) {
 // takes a token's heads `span` at a time, kRows of them loaded before the first is used.
 //   y = x rsqrt(mean(x^2) + eps) w,   out = y cos - y' sin  or  y cos + y' sin,   y' the partner's (i +- R/2, or the neighbour i ^ 1)
 // What depends on the channel and the token alone, w cos and the partner's w sin, is worked out once for all heads, so a channel costs a
-// product, a fused one and the row's factor (490 instructions for 8 rows of 128, half of what it was; N32760, 40 heads of 128 in q and k 412
+// product, a fused one and the row's factor (520 instructions for 8 rows of 128, half of what it was; N32760, 40 heads of 128 in q and k 412
 // -> 227 us, 5.9 TB/s, neighbours paired; halves 240).  All in fp32, one rounding to bf16.  To the cache goes the bf16 value, so that the fused and the separate form store the same bits: x = bf16(k - offset), scale =
 // e4m3(max|x| / 6) over the two lanes of a block, code = e2m1(x / scale).  Bound by DRAM.
 // ------------------------------------------------------------------------------------------------
