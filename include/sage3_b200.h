@@ -341,7 +341,8 @@ typedef struct {
   int32_t columns;
   int32_t is_causal;         /* bottom-right aligned per sequence                                              */
   float sm_scale;            /* <= 0: head_dim^-0.5                                                            */
-  void* workspace;           /* >= sage3_kv_attention_workspace bytes, 256-byte aligned; not shared by calls that can overlap  */
+  void* workspace;           /* >= sage3_kv_attention_workspace bytes, 256-byte aligned; not shared by calls that can overlap; may
+                                be NULL where that is 0                                                       */
   size_t workspace_bytes;
   int32_t* device_status;    /* optional device int32, zeroed by the call: the code of a bounded wait that gave up       */
 } sage3_kv_attention_args;

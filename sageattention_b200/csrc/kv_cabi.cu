@@ -132,7 +132,7 @@ int sage3_kv_attention_workspace(const sage3_kv_attention_args* a, size_t* bytes
 int sage3_kv_attention(const sage3_kv_attention_args* a, void* stream) {
   if (int st = check_attention(a)) return st;
   if (a->total_q == 0) return SAGE3_OK;
-  if (!a->q || !a->out || !a->kv_lens || !a->block_table || !a->workspace) return SAGE3_ERR_ARGUMENT;
+  if (!a->q || !a->out || !a->kv_lens || !a->block_table || (!a->workspace && a->workspace_bytes > 0)) return SAGE3_ERR_ARGUMENT;
   if (!aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->workspace, 256)) return SAGE3_ERR_ARGUMENT;
   if (a->q_stride_n % 8 || a->q_stride_h % 8 || a->out_stride_n % 8 || a->out_stride_h % 8) return SAGE3_ERR_ARGUMENT;
   if (a->cu_seqlens_q == nullptr && a->total_q < a->B) return SAGE3_ERR_ARGUMENT;

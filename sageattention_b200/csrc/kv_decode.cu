@@ -707,7 +707,7 @@ Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
   p.adds = p.starts + align256(items * 4);
   p.ml = p.adds + align256(items * 8 * p.nb * 4);
   p.o = p.ml + align256(p.ctas * 2 * 8 * p.nb * 8);
-  p.bytes = p.parts != 0 ? 256 : p.o + align256(p.ctas * 2 * 8 * p.nb * DS * 4);
+  p.bytes = p.parts != 0 ? 0 : p.o + align256(p.ctas * 2 * 8 * p.nb * DS * 4);
   return p;
 }
 
@@ -756,10 +756,13 @@ cudaError_t launch_kv_decode(const KvAttnArgs& a, cudaStream_t stream) {
   P.parts = p.parts; P.ctas = (int)p.ctas;
   P.page_shift = 0;
   while ((1 << P.page_shift) < a.page_size) ++P.page_shift;
-  char* const w = (char*)a.workspace;
-  P.header = (Header*)w;
-  P.item_start = (int*)(w + p.starts); P.lse_add = (float*)(w + p.adds);
-  P.ml_part = (float2*)(w + p.ml); P.o_part = (float*)(w + p.o);
+  P.header = nullptr; P.item_start = nullptr; P.lse_add = nullptr; P.ml_part = nullptr; P.o_part = nullptr;
+  if (p.bytes != 0) {
+    char* const w = (char*)a.workspace;
+    P.header = (Header*)w;
+    P.item_start = (int*)(w + p.starts); P.lse_add = (float*)(w + p.adds);
+    P.ml_part = (float2*)(w + p.ml); P.o_part = (float*)(w + p.o);
+  }
   const bool split = a.max_k > kBlock;     // else an item is one unit
   if (a.DS == 128) return p.nb == 1 ? launch<128, 1>(P, p, split, stream) : p.nb == 2 ? launch<128, 2>(P, p, split, stream) : launch<128, 3>(P, p, split, stream);
   return p.nb == 1   ? launch<64, 1>(P, p, split, stream)

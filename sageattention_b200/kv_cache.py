@@ -488,7 +488,6 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
         a.out_stride_h, a.out_stride_n = _strides(out)
     lse = torch.empty(plan.rows, dtype=torch.float32, device=dev) if return_lse else None
     if a.total_q:
-        ws = cache.data.new_empty(plan.workspace)
         qp = q.data_ptr()
         if qp & 15:
             _check_aligned(qp, "q")
@@ -497,7 +496,9 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
             a.lse = lse.data_ptr()
         if cu_seqlens_q is not None:
             a.cu_seqlens_q = cu_seqlens_q.data_ptr()
-        a.workspace = ws.data_ptr()
+        if plan.workspace:
+            ws = cache.data.new_empty(plan.workspace)
+            a.workspace = ws.data_ptr()
         status = torch.empty(1, dtype=torch.int32, device=dev) if check_status else None
         if status is not None:
             a.device_status = status.data_ptr()
