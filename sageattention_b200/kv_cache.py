@@ -463,8 +463,8 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     q: bf16 ``[tokens, Hq, head_dim]``, ``Hq`` a multiple of the cache's heads; sequence i has rows ``cu_seqlens_q[i] ... cu_seqlens_q[i+1]`` (int32
     ``[B+1]``), or row i alone where ``cu_seqlens_q`` is None.  ``kv_lens`` int32 ``[B]``: keys of each sequence, new ones included;
     ``block_table`` int32 ``[B, columns]``: their pages.  ``max_seqlen_q`` and ``max_seqlen_k`` (default: what the table can hold) must bound the
-    lengths - they size grid and workspace; rows and keys beyond them are left out.  ``is_causal``: bottom-right aligned, the last row of
-    a sequence sees all of its keys.
+    lengths - they size grid and workspace; rows and keys beyond them, or beyond q and the table, are left out.  ``is_causal``: bottom-right
+    aligned, the last row of a sequence sees all of its keys; the diagonal goes by the lengths as given, whatever is left out.
 
     Attention is over the values that the cache stands for, queries and softmax are not quantised.  Rows that see no key give zeros and an
     LSE of ``-inf``; keys of pages outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not

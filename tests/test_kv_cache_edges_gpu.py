@@ -1,0 +1,47 @@
+"""The 4-bit cache at its edges: lengths beyond what tables, bounds and outputs hold."""
+import numpy as np
+import pytest
+import torch
+
+import sageattention_b200 as sa
+from tests import _kv_reference as R
+from tests.test_kv_cache_gpu import BF, DEV, gen, make_cache, normal
+
+pytestmark = pytest.mark.gpu
+I32 = dict(dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("tokens,before", [(6, 200), (6, 9001), (150, 70), (150, 1300)])
+@pytest.mark.parametrize("what", ["columns", "max_seqlen_k", "max_seqlen_q", "rows of q"])
+def test_what_does_not_fit_is_left_out_and_moves_no_row(what, tokens, before, D):
+    """Keys beyond the table's columns or max_seqlen_k, and rows beyond max_seqlen_q or q, are not there; a row that is sees its own
+    place's keys as ever.  The reference takes each row as a sequence of its own."""
+    g = gen(tokens + before + D)
+    kv_lens, q_lens = [before + tokens, tokens, before // 2 + tokens], [tokens, tokens, tokens - 1]      # (the second: a prompt)
+    cache, table = make_cache(g, kv_lens, 2, D, 16, offset=True)
+    T, rows, max_q, keys = sum(q_lens), sum(q_lens), tokens, 16 * table.shape[1]
+    if what == "columns":
+        table = table[:, :(tokens // 2 if before < 100 else before + tokens // 2) // 16].contiguous()
+        keys = 16 * table.shape[1]
+    elif what == "max_seqlen_k":
+        keys = tokens // 2 + 1 if before < 100 else before + tokens // 2 - 3
+    elif what == "max_seqlen_q":
+        max_q = tokens - 2
+    else:
+        rows = T - 3
+    q = normal(g, rows, 4, D)
+    out = torch.full((rows, 4, D), 7.0, dtype=BF, device=DEV)
+    starts = np.concatenate(([0], np.cumsum(q_lens)))
+    got, lse = sa.sageattn_kvcache(q.to(DEV), cache, table.to(DEV), torch.tensor(kv_lens, **I32), torch.tensor(starts, **I32), max_q, keys,
+                                   return_lse=True, out=out, check_status=True)
+    owner = [b for b, n in enumerate(q_lens) for _ in range(n)][:rows]
+    place = [t for n in q_lens for t in range(n)][:rows]
+    there = np.array([t < max_q for t in place])
+    sees = [max(0, min(keys, kv_lens[b] - q_lens[b] + t + 1)) for b, t in zip(owner, place)]
+    want, wl, tol, ltol = R.attend(q, cache.data.cpu().numpy(), D, 16, [table[b].tolist() for b in owner], sees, [1] * rows, k_offset=cache.k_offset.cpu())
+    o, l = got.double().cpu().numpy(), lse.double().cpu().numpy()
+    assert (o[~there] == 7).all()
+    o, l, want, wl, tol, ltol = (x[there] for x in (o, l, want, wl, tol, ltol))
+    assert (np.abs(o - want) <= tol).all()
+    assert np.array_equal(np.isneginf(l), np.isneginf(wl)) and (np.abs(l - wl)[np.isfinite(wl)] <= ltol[np.isfinite(wl)]).all()
