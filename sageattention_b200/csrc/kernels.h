@@ -163,6 +163,7 @@ struct KvTablesArgs {                     // block tables and slots of a step (k
   int64_t* slots;                         // [num_tokens]
   int* taken;                             // [1]
 };
+constexpr int kTableMost = 16384;         // requests: their prefix sums lie in shared memory
 cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream);
 
 struct KvRows {                           // bf16 rows, element strides

@@ -58,7 +58,7 @@ int sage3_kv_block_tables(const sage3_kv_tables_args* a, void* stream) {
   if (!a->lens_before || !a->lens_new || !a->block_table || !a->kv_lens || !a->cu_seqlens_q || !a->pages_taken) return SAGE3_ERR_ARGUMENT;
   if ((a->num_free > 0 && !a->free_pages) || (a->num_tokens > 0 && (!a->positions || !a->slots))) return SAGE3_ERR_ARGUMENT;
   if (a->page_size != 16 && a->page_size != 32 && a->page_size != 64 && a->page_size != 128) return SAGE3_ERR_UNSUPPORTED;
-  if (a->B > 16384) return SAGE3_ERR_UNSUPPORTED;              // the prefix sums of all requests lie in shared memory
+  if (a->B > sage3::kTableMost) return SAGE3_ERR_UNSUPPORTED;
   sage3::KvTablesArgs k{};
   k.before = a->lens_before; k.fresh = a->lens_new; k.free_pages = a->free_pages;
   k.table = a->block_table; k.table_stride = a->row_stride;

@@ -103,9 +103,11 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const KvTab
 cudaError_t launch_block_tables(const KvTablesArgs& a, cudaStream_t stream) {
   int sms;
   if (cudaError_t e = sm_count(&sms); e != cudaSuccess) return e;
+  // The most that any call needs, whatever this one does: what a kernel may use belongs to the kernel, and a call with fewer requests must not
+  // take it from one that another thread is about to launch.  (Above 48 KB less the kernel's own 64 bytes it has to be asked for.)
+  static std::atomic<uint64_t> allowed;
+  if (cudaError_t e = allow_smem(block_tables_kernel, 2 * (kTableMost + 1) * (int)sizeof(int), allowed); e != cudaSuccess) return e;
   const int smem = 2 * (a.B + 1) * (int)sizeof(int);
-  if (smem > 48 * 1024)
-    if (cudaError_t e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return e;
   const int64_t work = (int64_t)a.num_tokens > a.B ? a.num_tokens : a.B;
   const int ctas = (int)((work + kTableThreads - 1) / kTableThreads);
   block_tables_kernel<<<ctas < sms ? ctas : sms, kTableThreads, smem, stream>>>(a);

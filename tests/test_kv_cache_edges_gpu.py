@@ -1,4 +1,8 @@
-"""The 4-bit cache at its edges: lengths beyond what tables, bounds and outputs hold."""
+"""The 4-bit cache at its edges: lengths beyond what tables, bounds and outputs hold, the most requests."""
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -45,3 +49,29 @@ def test_what_does_not_fit_is_left_out_and_moves_no_row(what, tokens, before, D)
     o, l, want, wl, tol, ltol = (x[there] for x in (o, l, want, wl, tol, ltol))
     assert (np.abs(o - want) <= tol).all()
     assert np.array_equal(np.isneginf(l), np.isneginf(wl)) and (np.abs(l - wl)[np.isfinite(wl)] <= ltol[np.isfinite(wl)]).all()
+
+
+SHARED = """
+import torch, sageattention_b200 as sa
+from concurrent.futures import ThreadPoolExecutor
+i32 = dict(dtype=torch.int32, device="cuda")
+
+def one(B):
+    new = torch.arange(B, **i32) % 3
+    r = sa.build_block_tables(torch.zeros(B, **i32), new, torch.full((B, 1), -1, **i32), torch.arange(B, **i32), 16, 4)
+    want = torch.cat((new.new_zeros(1), new.cumsum(0)))
+    assert torch.equal(r.cu_seqlens_q.long(), want), B
+
+for B in (6135, 6136, 6143, 6144, 6136, 16384, 6136):          # no larger one before the first four
+    one(B)
+with ThreadPoolExecutor(2) as pool:
+    list(pool.map(one, [16384, 6200] * 200))
+torch.cuda.synchronize()
+print("fine")
+"""
+
+
+def test_block_tables_of_as_many_requests_as_shared_memory_holds():
+    """In a process of its own: what the kernel may use is set once."""
+    r = subprocess.run([sys.executable, "-c", SHARED], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
