@@ -139,12 +139,24 @@ __device__ __forceinline__ uint32_t quant_codes(const uint4& x, float inv) {
   }
   return f32x8_to_e2m1x8(f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y);
 }
+// A block's largest channel, of which a NaN anywhere in the block makes a NaN: its scale then is the NaN of E4M3, and so is all that is read back.
+// (The conversion to codes has no NaN and would leave a plausible number.)  Per half of the words max(|a|, |b|); the sign is of no meaning.
+__device__ __forceinline__ uint32_t nan_habsmax2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t nan_habsmax2(const uint4& x) { return nan_habsmax2(nan_habsmax2(x.x, x.y), nan_habsmax2(x.z, x.w)); }
+__device__ __forceinline__ float nan_absmax(uint32_t x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(bf16_lo(abs2(x))), "f"(bf16_hi(abs2(x))));
+  return r;
+}
 // Codes and scale (of a block of 16 channels, whose other half the next lane has)
 __device__ __forceinline__ void quant_half_block(const uint4& x, uint32_t& codes, uint32_t& scale) {
-  uint32_t m2 = abs2(habsmax2(habsmax2(x.x, x.y), habsmax2(x.z, x.w)));
-  m2 = abs2(habsmax2(m2, __shfl_xor_sync(0xffffffffu, m2, 1)));
+  const uint32_t m2 = nan_habsmax2(x);
   float inv;
-  block_scale(fmaxf(bf16_lo(m2), bf16_hi(m2)), scale, inv);     // (its approximate operations are exact on bf16: tests/golden/device_tables)
+  block_scale(nan_absmax(nan_habsmax2(m2, __shfl_xor_sync(0xffffffffu, m2, 1))), scale, inv);     // (its approximate operations are exact on bf16: tests/golden/device_tables)
   codes = quant_codes(x, inv);
 }
 
@@ -380,10 +392,9 @@ __global__ void __launch_bounds__(kTokenThreads) kv_append_kernel(const KvTokens
 #pragma unroll
   for (int what = 0; what < 2; ++what) {
     const uint4 u = x[what][0], v = x[what][1];
-    const uint32_t m2 = abs2(habsmax2(habsmax2(habsmax2(u.x, u.y), habsmax2(u.z, u.w)), habsmax2(habsmax2(v.x, v.y), habsmax2(v.z, v.w))));
     uint32_t scale;
     float inv;
-    block_scale(fmaxf(bf16_lo(m2), bf16_hi(m2)), scale, inv);
+    block_scale(nan_absmax(nan_habsmax2(nan_habsmax2(u), nan_habsmax2(v))), scale, inv);
     const uint2 codes = make_uint2(quant_codes(u, inv), quant_codes(v, inv));
     if (what == 0) {
       *reinterpret_cast<uint2*>(p.rec + Rec::key(p.t, blk * 16)) = codes;

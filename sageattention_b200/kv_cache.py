@@ -166,7 +166,8 @@ class FP4KVCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Writes k, v (bf16 ``[T, num_kv_heads, head_dim]``) to the slots (int64 ``[T]``) ``page * page_size + place``.  Slots outside the cache
-        (-1) are skipped; a slot named twice ends up with a mixture of its tokens."""
+        (-1) are skipped; a slot named twice ends up with a mixture of its tokens.  A NaN makes its block of 16 channels NaN, infinities become
+        the block's largest number."""
         key = ("kv_append", _sig(k), _sig(v), self._key)
         plan = _plans.get(key)
         if plan is None or not _is(slots, torch.int64, plan.rows, self.device):
@@ -467,7 +468,8 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     aligned, the last row of a sequence sees all of its keys; the diagonal goes by the lengths as given, whatever is left out.
 
     Attention is over the values that the cache stands for, queries and softmax are not quantised.  Rows that see no key give zeros and an
-    LSE of ``-inf``; keys of pages outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not
+    LSE of ``-inf``; a row that sees a key or value with a NaN in it may be NaN altogether, and others are not touched by it; keys of pages
+    outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not
     touched in ``out`` (or are undefined in a new tensor).  Returns the output like q, and with ``return_lse`` the natural-log LSE fp32
     ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where one of their bounded waits gave up."""
     if out is not None:

@@ -1,4 +1,4 @@
-"""The 4-bit cache at its edges: lengths beyond what tables, bounds and outputs hold, the most requests."""
+"""The 4-bit cache at its edges: lengths beyond what tables, bounds and outputs hold, the most requests, numbers that are none."""
 import subprocess
 import sys
 from pathlib import Path
@@ -75,3 +75,46 @@ def test_block_tables_of_as_many_requests_as_shared_memory_holds():
     """In a process of its own: what the kernel may use is set once."""
     r = subprocess.run([sys.executable, "-c", SHARED], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
     assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("D", [128, 64, 72, 8])
+def test_a_lone_nan_marks_its_block(D):
+    """One NaN among finite channels (and beside the padding of a head dim that is no multiple of 16): the block reads back as NaN, and
+    all others as they would without it."""
+    g = gen(61 + D)
+    T, H = 40, 2
+    k, v = normal(g, T, H, D), normal(g, T, H, D)
+    hit = torch.zeros(2, T, H, D, dtype=torch.bool)
+    for i in range(T // 2):                                    # every channel in turn, and two in one block
+        hit[i % 2, 2 * i, i % H, (7 * i) % D] = True
+    hit[0, 1, 0, D - 1] = hit[0, 1, 0, D - 3] = True
+    bad = [torch.where(h, torch.full_like(x, float("nan")), x) for h, x in zip(hit, (k, v))]
+    slots = torch.randperm(64, generator=g)[:T].to(DEV)
+    got, clean = [], []
+    for res, (a, b) in ((got, bad), (clean, (k, v))):
+        cache = sa.FP4KVCache.empty(4, H, D, 16)
+        cache.append(a.to(DEV), b.to(DEV), slots)
+        res += [t.cpu() for t in cache.read(slots)]
+        fused = sa.FP4KVCache.empty(4, H, D, 16)               # the kernel with queries writes the same
+        sa.qk_norm_rope_append(a[:, :1].to(DEV), a.to(DEV), b.to(DEV), fused, slots)
+        assert all(torch.equal(x.nan_to_num(7e4), y.nan_to_num(7e4)) for x, y in zip((t.cpu() for t in fused.read(slots)), res[-2:]))
+    for x, y, h in zip(got, clean, hit):
+        pad = -D % 16
+        block = torch.nn.functional.pad(h, (0, pad)).unflatten(-1, (-1, 16)).any(-1, keepdim=True).expand(T, H, (D + pad) // 16, 16).flatten(-2)[..., :D]
+        assert x[block].isnan().all() and torch.equal(x[~block], y[~block])
+
+
+@pytest.mark.parametrize("rot", [8, 24, 64])
+def test_keys_of_positions_outside_the_table_are_nan(rot):
+    """Also where the rotated channels end in the middle of a block."""
+    g = gen(rot)
+    q, k, v = normal(g, 4, 2, 64).to(DEV), normal(g, 4, 1, 64).to(DEV), normal(g, 4, 1, 64).to(DEV)
+    cos, sin = torch.ones(3, rot // 2, device=DEV), torch.zeros(3, rot // 2, device=DEV)
+    cache, slots = sa.FP4KVCache.empty(1, 1, 64, 16), torch.arange(4, device=DEV)
+    sa.qk_norm_rope_append(q, k, v, cache, slots, cos, sin, torch.tensor([0, 3, 2, -1], device=DEV))
+    rk, rv = cache.read(slots)
+    end = -(-rot // 16) * 16
+    assert rk[[1, 3], :, :end].isnan().all() and rk[[1, 3], :, end:].isfinite().all() and rk[[0, 2]].isfinite().all() and rv.isfinite().all()
+    lens = torch.tensor([1, 2], **I32)
+    o = sa.sageattn_kvcache(q[:2], cache, torch.zeros(2, 1, **I32), lens)
+    assert o[0].isfinite().all() and o[1].isnan().all()
