@@ -109,8 +109,8 @@ int sage3_kv_read(const sage3_kv_cache* cache, const int64_t* slots, int64_t T, 
   if (int st = check_cache(cache)) return st;
   if (T < 0) return SAGE3_ERR_ARGUMENT;
   if (T == 0) return SAGE3_OK;
+  if (T >= (1ll << 31) - 64 || cache->num_kv_heads > 32767) return SAGE3_ERR_UNSUPPORTED;      // (a CTA counts up to 63 tokens beyond the last)
   if (!slots || !k || !v || !aligned(k, 16) || !aligned(v, 16)) return SAGE3_ERR_ARGUMENT;
-  if (T >= (1ll << 31) || cache->num_kv_heads > 32767) return SAGE3_ERR_UNSUPPORTED;
   sage3::KvReadArgs a{};
   a.data = (const uint8_t*)cache->data; a.slots = slots; a.T = T; a.num_slots = cache->num_pages * cache->page_size;
   a.Hkv = cache->num_kv_heads; a.D = cache->head_dim; a.DS = cache->head_dim_stored; a.page_shift = shift_of(cache->page_size);

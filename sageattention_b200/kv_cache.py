@@ -192,6 +192,7 @@ class FP4KVCache:
         if T < 0 or slots.dtype != torch.int64 or slots.device != self.device or not slots.is_contiguous():
             _require(T >= 0, "slots must be [tokens]")
             _check_ids("slots", slots, torch.int64, slots.shape, self.device)
+        _require(T < 2 ** 31 - 64, "too many tokens for one call")
         dev = self.device
         _check_b200(dev, self.data)
         k = torch.empty((T, self.num_kv_heads, self.head_dim), dtype=torch.bfloat16, device=dev)

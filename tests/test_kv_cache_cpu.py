@@ -321,3 +321,13 @@ def test_numbers_of_tables_and_rotation():
         sa.build_block_tables(**table_args(num_tokens=torch.tensor(3)))
     with pytest.raises(ValueError, match="not a tensor"):
         sa.qk_norm_rope(**rope_args(eps=torch.tensor(1e-6)))
+
+
+def test_reading_more_tokens_than_the_kernel_counts():
+    """Token numbers of the last, partly filled CTA must not pass 2^31."""
+    c = _lib.KvCache(1 << 12, 4, 2, 16, 64, 64, None)
+    for T in (2 ** 31 - 64, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        assert _lib.load().sage3_kv_read(C.byref(c), 1 << 12, T, 1 << 12, 1 << 12, None) == _lib.ERR_UNSUPPORTED, T
+    meta = sa.FP4KVCache.empty(4, 2, 64, 16, device="meta")
+    with pytest.raises(ValueError, match="too many"):
+        meta.read(torch.empty(2 ** 31 - 64, dtype=torch.int64, device="meta"))
