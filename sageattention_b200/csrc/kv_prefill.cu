@@ -98,14 +98,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
                  "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(taddr) : "memory");
 }
-// Waits for the tensor-memory loads under way; names the registers, so that nothing that reads them can be moved in front of it.
-__device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
-                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
-               :: "memory");
-  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+// A load's registers may be read once tcgen05.wait::ld is behind it.  Naming them here, behind the wait, ties their readers to it: to the compiler
+// they are written by the load, and nothing else keeps a reader from being moved in front of the wait.
+template <int N>
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 16)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]),
+                      "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]), "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15]));
 }
 // fp16 x fp16 -> fp32, A K-major, B K-major or (transposed) MN-major
 __host__ __device__ constexpr uint32_t idesc_f16(int N, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kM >> 4) << 24); }
@@ -448,6 +448,8 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
 #pragma unroll
       for (int i = 0; i < 4; ++i) tmem_ld32(tm_s + 32 * i, s[i]);
       tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_loaded(s[i]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + Bar::s_free + 8 * (kSBufs == 1 ? 0 : t));
@@ -505,6 +507,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
             uint32_t o[16];
             tmem_ld16(tm_o + 16 * i, o);
             tmem_wait_ld();
+            tmem_loaded(o);
 #pragma unroll
             for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
             tmem_st16(tm_o + 16 * i, o);
@@ -538,6 +541,7 @@ __global__ void __launch_bounds__(kThreads2, 1) kv_prefill_kernel(const Params2 
         if (count > 0) {
           tmem_ld32(tm_o + 32 * i, o);
           tmem_wait_ld();
+          tmem_loaded(o);
         } else {
 #pragma unroll
           for (int x = 0; x < 32; ++x) o[x] = 0;
