@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kTokenThreads, 4) kv_tokens_kernel(const KvTok
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       x[p] = make_uint4(0, 0, 0, 0);
-      if (have && first + p * kPerPass + sub < h1) x[p] = __ldg(reinterpret_cast<const uint4*>(from));
+      if (have && first + p * kPerPass + sub < h1) x[p] = *reinterpret_cast<const uint4*>(from);      // (no __ldg: outputs may be the inputs)
       from += from_step;
     }
   };

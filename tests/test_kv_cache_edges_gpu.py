@@ -118,3 +118,16 @@ def test_keys_of_positions_outside_the_table_are_nan(rot):
     lens = torch.tensor([1, 2], **I32)
     o = sa.sageattn_kvcache(q[:2], cache, torch.zeros(2, 1, **I32), lens)
     assert o[0].isfinite().all() and o[1].isnan().all()
+
+
+@pytest.mark.parametrize("D,heads,adjacent", [(128, 40, True), (64, 40, False), (128, 9, False)])
+def test_norm_rope_in_place_over_many_rows(D, heads, adjacent):
+    """A warp goes over a token's heads a few at a time, in a fused projection's own memory."""
+    g = gen(D + heads)
+    x = normal(g, 5000, 2 * heads + 1, D).to(DEV)
+    cos, sin = (torch.randn(5000, D // 2, generator=g).to(DEV) for _ in range(2))
+    w = normal(g, D).to(DEV)
+    q, k, rest = x[:, :heads], x[:, heads:2 * heads], x[:, 2 * heads:].clone()
+    want = sa.qk_norm_rope(q, k, cos, sin, None, w, w, adjacent_pairs=adjacent)
+    got = sa.qk_norm_rope(q, k, cos, sin, None, w, w, adjacent_pairs=adjacent, out=(q, k))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is q and torch.equal(x[:, 2 * heads:], rest)
