@@ -384,6 +384,11 @@ def _norm_rope_pointers(a, q, k, cos, sin, positions, q_weight, k_weight):
 def _check_out(o, x):
     _check_bf16(o)
     _require(o.shape == x.shape and o.device == x.device, "outputs must have the shapes and device of the inputs")
+    end = 0                                                         # of the elements that the dimensions so far reach
+    for step, n in sorted(zip(o.stride(), o.shape)):
+        if n > 1:
+            _require(step > end, "elements of an output must not lie on one another")
+            end += step * (n - 1)
     _check_rows(o)
     _check_aligned(o.data_ptr(), "outputs")
 
@@ -399,7 +404,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
     weight``, or no norm where None.  ``cos``, ``sin`` (fp32 ``[positions, rot_dim / 2]``): the first ``rot_dim`` channels are rotated, pairs being
     ``(i, i + rot_dim / 2)``, or ``(2i, 2i + 1)`` with ``adjacent_pairs``.  ``positions``: int32 or int64 ``[tokens]`` (``[batch, tokens]``), default
     0, 1, ... in each batch entry; one outside the table gives NaN.  All in fp32, rounded once.  ``out``: the two outputs, which may be q and
-    k themselves."""
+    k themselves (each its own); else they share no memory with them."""
     if out is not None:
         _check_out(out[0], q)
         _check_out(out[1], k)
@@ -426,7 +431,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache
                         k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, adjacent_pairs: bool = False,
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`qk_norm_rope` of ``[tokens, heads, head_dim]`` tensors with the keys, and the values as they are, written straight to the cache
-    (the same bits as :meth:`FP4KVCache.append` of its result).  Returns the queries."""
+    (the same bits as :meth:`FP4KVCache.append` of its result).  Returns the queries; ``out``, for them, may be q itself."""
     if out is not None:
         _check_out(out, q)
     key = _norm_rope_key("qk_norm_rope_append", q, k, cos, positions, q_weight, k_weight, eps, adjacent_pairs, None, v.shape, v.stride(), v.dtype,
@@ -471,7 +476,7 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     Attention is over the values that the cache stands for, queries and softmax are not quantised.  Rows that see no key give zeros and an
     LSE of ``-inf``; a row that sees a key or value with a NaN in it may be NaN altogether, and others are not touched by it; keys of pages
     outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not
-    touched in ``out`` (or are undefined in a new tensor).  Returns the output like q, and with ``return_lse`` the natural-log LSE fp32
+    touched in ``out`` (or are undefined in a new tensor), which shares no memory with the inputs.  Returns the output like q, and with ``return_lse`` the natural-log LSE fp32
     ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where one of their bounded waits gave up."""
     if out is not None:
         _check_out(out, q)

@@ -331,3 +331,21 @@ def test_reading_more_tokens_than_the_kernel_counts():
     meta = sa.FP4KVCache.empty(4, 2, 64, 16, device="meta")
     with pytest.raises(ValueError, match="too many"):
         meta.read(torch.empty(2 ** 31 - 64, dtype=torch.int64, device="meta"))
+
+
+def test_outputs_whose_elements_lie_on_one_another():
+    wide = torch.zeros(3, 1, 64, dtype=BF).expand(3, 4, 64)
+    steps = torch.zeros(512, dtype=BF).as_strided((3, 4, 64), (64, 8, 1))
+    for bad in (wide, steps, torch.zeros(1, 4, 64, dtype=BF).expand(3, 4, 64)):
+        with pytest.raises(ValueError, match="on one another"):
+            sa.qk_norm_rope(**rope_args(out=(bad, tokens())))
+        with pytest.raises(ValueError, match="on one another"):
+            sa.qk_norm_rope_append(tokens(H=4), tokens(), tokens(), cache(), ints(0, 1, 2, dtype=torch.int64), out=bad)
+        with pytest.raises(ValueError, match="on one another"):
+            sa.sageattn_kvcache(**attention_args(q=tokens(T=3, H=4), out=bad))
+    # slices, other orders of dimensions and dimensions of one are fine: the device is looked at next
+    for good in (torch.zeros(3, 9, 80, dtype=BF)[:, 2:6, :64], torch.zeros(4, 3, 64, dtype=BF).transpose(0, 1)):
+        with pytest.raises(ValueError, match="CUDA tensors only"):
+            sa.qk_norm_rope(**rope_args(out=(good, tokens())))
+    with pytest.raises(ValueError, match="CUDA tensors only"):
+        sa.qk_norm_rope(**rope_args(q=tokens(T=1, H=1), k=tokens(T=1), out=(torch.zeros(64, dtype=BF).as_strided((1, 1, 64), (0, 0, 1)), tokens(T=1))))
