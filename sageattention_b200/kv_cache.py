@@ -403,7 +403,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] =
     a fused projection); head_dim a multiple of 8 up to 128.  ``q_weight``, ``k_weight`` (bf16 ``[head_dim]``): ``x * rsqrt(mean(x^2) + eps) *
     weight``, or no norm where None.  ``cos``, ``sin`` (fp32 ``[positions, rot_dim / 2]``): the first ``rot_dim`` channels are rotated, pairs being
     ``(i, i + rot_dim / 2)``, or ``(2i, 2i + 1)`` with ``adjacent_pairs``.  ``positions``: int32 or int64 ``[tokens]`` (``[batch, tokens]``), default
-    0, 1, ... in each batch entry; one outside the table gives NaN.  All in fp32, rounded once.  ``out``: the two outputs, which may be q and
+    0, 1, ... in each batch entry; one outside the table gives NaN.  All in fp32, rounded once: a norm needs squares that fp32 holds (channels up
+    to 1e18; a row beyond gives zeros or NaN).  ``out``: the two outputs, which may be q and
     k themselves (each its own); else they share no memory with them."""
     if out is not None:
         _check_out(out[0], q)
