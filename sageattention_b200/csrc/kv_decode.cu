@@ -561,21 +561,28 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(D, NB)) kv_decode_ker
     int b = where_s[0];
     int rest = unit - where_s[1];            // units of sequence b before this one
 
+    // Each round has the same barriers for all warps and ends by a vote, so that all take as many, whatever each has read of lengths that another
+    // stream writes meanwhile.
 #pragma unroll 1
-    while (unit < unit_end) {
-      const KvSeq seq(A, b);
-      const int blocks = blocks_of(seq), tiles = tiles_of<kRows>(seq, P.group);
-      if (rest >= A.Hkv * tiles * blocks) {             // on to the next sequence
-        rest -= A.Hkv * tiles * blocks;
-        if (++b >= A.B) break;
-        continue;
+    do {
+      for (;;) {
+        const KvSeq seq(A, b);
+        const int blocks = blocks_of(seq), tiles = tiles_of<kRows>(seq, P.group);
+        if (rest >= A.Hkv * tiles * blocks) {           // on to the next sequence
+          rest -= A.Hkv * tiles * blocks;
+          if (++b < A.B) continue;
+          unit = unit_end;                               // (there is none: lengths have changed)
+          __syncthreads();                               // as in an item
+          __syncthreads();
+          break;
+        }
+        const int item = rest / blocks, block = rest - item * blocks, take = min(blocks - block, unit_end - unit), h = item / tiles, tile = item - h * tiles;
+        item_part(seq, b, h, tile, block, take, blocks, unit);
+        unit += take;
+        rest += take;
+        break;
       }
-      const int item = rest / blocks, block = rest - item * blocks, take = min(blocks - block, unit_end - unit), h = item / tiles, tile = item - h * tiles;
-      item_part(seq, b, h, tile, block, take, blocks, unit);
-      unit += take;
-      rest += take;
-      __syncthreads();                       // the ring is the next item's
-    }
+    } while (__syncthreads_and(unit < unit_end));        // (and the ring is the next item's)
   }
 }
 
