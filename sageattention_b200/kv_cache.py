@@ -475,7 +475,8 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     aligned, the last row of a sequence sees all of its keys; the diagonal goes by the lengths as given, whatever is left out.
 
     Attention is over the values that the cache stands for, queries and softmax are not quantised.  Rows that see no key give zeros and an
-    LSE of ``-inf``; a row that sees a key or value with a NaN in it may be NaN altogether, and others are not touched by it; keys of pages
+    LSE of ``-inf``; a row that sees a key or value with a NaN in it may be NaN altogether, and others are not touched by it (so may rows
+    whose scores pass 9e7 in size); keys of pages
     outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not
     touched in ``out`` (or are undefined in a new tensor), which shares no memory with the inputs.  Returns the output like q, and with ``return_lse`` the natural-log LSE fp32
     ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where one of their bounded waits gave up."""

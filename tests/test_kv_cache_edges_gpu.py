@@ -9,7 +9,7 @@ import torch
 
 import sageattention_b200 as sa
 from tests import _kv_reference as R
-from tests.test_kv_cache_gpu import BF, DEV, gen, make_cache, normal
+from tests.test_kv_cache_gpu import BF, DEV, check, gen, make_cache, normal
 
 pytestmark = pytest.mark.gpu
 I32 = dict(dtype=torch.int32, device=DEV)
@@ -131,3 +131,36 @@ def test_norm_rope_in_place_over_many_rows(D, heads, adjacent):
     want = sa.qk_norm_rope(q, k, cos, sin, None, w, w, adjacent_pairs=adjacent)
     got = sa.qk_norm_rope(q, k, cos, sin, None, w, w, adjacent_pairs=adjacent, out=(q, k))
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0] is q and torch.equal(x[:, 2 * heads:], rest)
+
+
+@pytest.mark.parametrize("D,tokens", [(64, 1), (128, 5), (64, 7), (128, 140)])
+def test_outputs_of_the_callers_own(D, tokens):
+    """Rows and heads further apart than they are long, in another order too: the bits of a call without ``out``, and nothing between them."""
+    g = gen(71 + tokens)
+    kv_lens, q_lens = [tokens + 300, tokens, 2500], [tokens, max(1, tokens - 1), tokens]
+    cache, table = make_cache(g, kv_lens, 2, D, 32)
+    T = sum(q_lens)
+    q, cu = normal(g, T + 2, 4, D).to(DEV), torch.tensor(np.concatenate(([0], np.cumsum(q_lens))), **I32)
+    args = (cache, table.to(DEV), torch.tensor(kv_lens, **I32), cu, tokens)
+    want, lse = sa.sageattn_kvcache(q, *args, return_lse=True)
+    for order in (False, True):
+        wide = torch.full((T + 2, 9, D + 24) if not order else (9, T + 2, D + 24), 7.0, dtype=BF, device=DEV)
+        inner = wide[:, 1:9:2, 8:D + 8] if not order else wide[1:9:2, :, 8:D + 8].transpose(0, 1)
+        got, l2 = sa.sageattn_kvcache(q, *args, return_lse=True, out=inner)
+        assert got is inner and torch.equal(inner[:T], want[:T]) and torch.equal(l2[:T], lse[:T])
+        inner[:T] = 7
+        assert (wide == 7).all()
+
+
+@pytest.mark.parametrize("D,tokens", [(128, 1), (64, 6), (128, 60)])
+def test_scores_as_large_as_they_may_be(D, tokens):
+    """Scores near 9e7: the rounding of a maximum's product with the scale, 8 and more there, still leaves weights within fp16."""
+    g = gen(73)
+    cache, table = make_cache(g, [700], 1, D, 32, outlier=8.0)
+    q = normal(g, tokens, 2, D) * 2.0 ** 17
+    kk, _ = R.values(cache.data.cpu().numpy(), D, 32)
+    keys = kk[table[0, torch.arange(700) // 32].numpy(), 0, np.arange(700) % 32]
+    for size in (1e5, 1e7, 8.5e7):
+        scale = size / np.abs(q.double().numpy() @ keys.T).max()
+        out, lse = check(q.to(DEV), cache, table, [700], [tokens], scale=scale)
+        assert out.isfinite().all() and lse.isfinite().all()
