@@ -13,7 +13,8 @@
 // programmatic dependent), are joined by their maxima and sums in a fixed order.
 //
 // What bounds it: a key costs D 9/8 bytes and, whatever the rows, the instructions that turn its codes into fp16.  32 sequences of 8192 keys, 32
-// heads of 8, D=128: 62 us, 4.9 TB/s; the chip's copy does 6.5.  Short caches are bound by latency: 1000 keys of one sequence 5.2 us.
+// heads of 8, D=128: 60.8 us, 5.0 TB/s; of 16384 108.8, so that long caches stream at 6.3 (the chip's copy does 6.5) and some 12 us are what
+// items cost at their start and end.  Short caches are bound by latency: 1000 keys of one sequence 6.3 us.
 #include "kernels.h"
 #include "kv_attn.cuh"
 
@@ -701,10 +702,13 @@ Plan plan(int B, int Hq, int Hkv, int DS, int max_q, int max_k, int sms) {
   p.rows = items * 8 * p.nb;
   p.ctas = p.units < fit ? p.units : fit;
   // A cluster (or a CTA) per item or equal runs?  Clusters are as large as all of them fit at once; a CTA's way through the keys must not be
-  // long beside an equal share of all of them, nor the last round of CTAs nearly empty.  us, equal runs -> clusters, 32 heads of 8, D=128, "~":
-  // lengths up to that.  One token: B1 1000 keys 6.4 -> 5.2, B12 4096 21.0 -> 16.9, B32 ~2048 20.0 -> 17.1, B64 ~1000 20.9 -> 16.8, B256 ~1000
-  // 66.8 -> 46.6, B128 4096 112.5 -> 104.2; 4 tokens: B16 ~4096 38 -> 29, B128 ~1000 72.6 -> 45.1; 6 tokens: B16 ~4096 53 -> 33.
-  // What the rule leaves to equal runs: B1 16384 12.8 -> 16.6, B20 ~8192 31 -> 36, B40 ~8192 47 -> 76.  One block needs no joining (4.1 -> 4.6).
+  // long beside an equal share of all of them, nor the last round of CTAs nearly empty.  us, equal runs -> clusters, lengths up to what is said, one
+  // token unless it says more.  32 heads of 8, D=128: B1 1000 keys 6.6 -> 6.7, B4 8192 15.1 -> 13.9, B12 4096 16.6 -> 14.1, B32 2048 17.6 -> 16.0,
+  // B64 1000 20.4 -> 15.9, B256 1000 57.8 -> 49.4, B128 1000 of 4 tokens 52.4 -> 48.6; D=64: B12 4096 12.8 -> 10.5, B64 1000 15.8 -> 11.5, B256 1000
+  // 40.6 -> 35.2; 16 heads of 16: B64 1000 D=128 31.1 -> 27.0, D=64 22.5 -> 19.5; 8 heads of 1, D=128: B256 1000 16.6 -> 12.3.
+  // What the rule leaves to equal runs: 32 heads of 8, B1 16384 12.5 -> 18.1, B40 8192 48.5 -> 68.2, D=64 32.9 -> 47.2; 16 heads of 16, B1 16384 15.0 ->
+  // 21.6; 8 heads of 1, B4 8192 9.2 -> 12.3.  Of 46 such shapes it takes the slower one by 8 % at most (8 heads of 1, B12 4096: 9.1 in place of 8.4).
+  // One block needs no joining (4.1 -> 4.6).
   p.parts = kMostParts;
   while (p.parts > 1 && (items * p.parts > fit || p.parts >= 2 * blocks)) p.parts /= 2;
   const int64_t longest = (blocks + p.parts - 1) / p.parts;

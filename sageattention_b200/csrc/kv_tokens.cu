@@ -9,8 +9,8 @@ namespace sage3 {
 // Block tables.  With have = ceil(before / ps), need = ceil((before + new) / ps) - have and their exclusive sums, new page number e of
 // the step belongs to the request that a search in the sums finds, and so does token t.  One launch: every CTA scans all requests
 // (8 bytes each, from L2) into shared memory and then takes its share of pages and tokens, so that one request with a long
-// prompt costs no more than many with short ones.  Bound by its latencies, a chain of loads and barriers: 48 requests of one
-// token 3.0 us, 700 requests and 1e5 tokens 8.7 us.
+// prompt costs no more than many with short ones.  Bound by its latencies, a chain of loads, barriers and searches, and by divisions by the page
+// size, four for every request, page and token: 48 requests of one token 3.0 us, 700 requests and 1e5 tokens 8.7 us.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTableThreads = 256;
 
@@ -355,7 +355,8 @@ cudaError_t launch_kv_tokens(KvTokensArgs a, cudaStream_t stream) {
 // ------------------------------------------------------------------------------------------------
 // Keys and values as they are into the cache, and back.  A thread has a whole block of 16 channels, a warp 4 (8) tokens next to one
 // another of a head: their values' codes lie in the same 32-byte sectors.  Blocks a thread has alone need no exchange, and a scale is
-// worked out once for 16 channels (20011 tokens, 8 heads of 128: 16.7 us, 6.3 TB/s, against 31 with 8 channels a lane as above; back 20.5 against 25).
+// worked out once for 16 channels (20011 tokens, 8 heads of 128, repeated with the writes in L2: 16.7 us against 31 with 8 channels a lane as above, back
+// 20.5 against 25; with the writes going out 19.6 and 23.1).
 // Slots outside the cache are skipped, and give zeros.
 // ------------------------------------------------------------------------------------------------
 struct Place {

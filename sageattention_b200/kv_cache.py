@@ -475,11 +475,13 @@ def sageattn_kvcache(q: torch.Tensor, cache: FP4KVCache, block_table: torch.Tens
     aligned, the last row of a sequence sees all of its keys; the diagonal goes by the lengths as given, whatever is left out.
 
     Attention is over the values that the cache stands for, queries and softmax are not quantised.  Rows that see no key give zeros and an
-    LSE of ``-inf``; a row that sees a key or value with a NaN in it may be NaN altogether, and others are not touched by it (so may rows
-    whose scores pass 9e7 in size); keys of pages
-    outside the cache (-1) are not seen; rows of q that belong to no sequence (a padded batch) are not
-    touched in ``out`` (or are undefined in a new tensor), which shares no memory with the inputs.  Returns the output like q, and with ``return_lse`` the natural-log LSE fp32
-    ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where one of their bounded waits gave up."""
+    LSE of ``-inf``.  A row that sees a key or value with a NaN in it may be NaN altogether, others are not touched by it; scores (``sm_scale * q.k``)
+    beyond 9e7 in size give NaN or zeros.  Keys of pages outside the cache (-1) are not seen.  Rows of q that belong to no sequence (a padded
+    batch) are not touched in ``out``, or are undefined in a new tensor; ``out`` shares no memory with the inputs.  Returns the output like q, and
+    with ``return_lse`` the natural-log LSE fp32 ``[tokens, Hq]`` of ``sm_scale * q.k``.  ``check_status`` waits for the kernels and raises where
+    one of their bounded waits gave up.
+
+    The longest request picks the kernel: where some bring many tokens and others one, two calls, each with its own rows, are faster."""
     if out is not None:
         _check_out(out, q)
     # (what the launch is made for goes by blocks of 128 keys: a plan lasts for as many steps)
