@@ -328,7 +328,8 @@ typedef struct {
 
 typedef struct {
   const sage3_kv_cache* cache;
-  int32_t B, Hq, max_seqlen_q, max_seqlen_k, total_q;   /* max_*: bounds on the lengths; rows of q: total_q     */
+  int32_t B, Hq, max_seqlen_q, max_seqlen_k, total_q;   /* max_*: bounds on the lengths; rows of q: total_q. Rows and keys
+                                beyond these, or beyond the table, are left out and move no other row           */
   const void* q;             /* bf16 [total_q, Hq, head_dim], strides in elements                              */
   int64_t q_stride_n, q_stride_h;
   void* out;                 /* likewise; rows of no sequence stay as they are                                 */
